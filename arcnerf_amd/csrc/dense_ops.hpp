@@ -1,0 +1,114 @@
+// DenseOps<T>: one translation unit per element type includes this and instantiates it.
+#pragma once
+
+#include "dense.hpp"
+
+namespace arcn {
+
+template <typename T>
+static const T *tp(const void *p) {
+    return static_cast<const T *>(p);
+}
+
+template <typename T>
+int DenseOps<T>::fwd(const void *x, int64_t ld_x, const void *w, const void *b, const void *res, int64_t ld_res, void *y, int act, float beta, int64_t rows, int K, int N,
+                     hipStream_t st) {
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(w), nullptr, K, N, K, 0};
+    p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
+    p.bias = tp<T>(b);
+    p.res = tp<T>(res);
+    p.ld_res = ld_res;
+    p.out = static_cast<T *>(y);
+    p.ld_out = N;
+    p.act = act;
+    p.beta = beta;
+    if (rows <= kFewRows) {
+        const dim3 grid((unsigned)ceil_div<int>(N, 16));
+        if (rows <= 16) hipLaunchKernelGGL((dense_few_kernel<T, false, 1>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((dense_few_kernel<T, false, 2>), grid, dim3(256), 0, st, p);
+        return check_launch("dense_fwd");
+    }
+    return launch_tiles<T, kDenseFwd>(p, st);
+}
+
+template <typename T>
+int DenseOps<T>::dz(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, int act, float beta, int64_t rows, int K, int N,
+                    hipStream_t st) {
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(w), nullptr, K, N, K, 0};
+    p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
+    p.bias = tp<T>(b);
+    p.res = tp<T>(dy);
+    p.ld_res = ld_dy;
+    p.out = static_cast<T *>(dz);
+    p.ld_out = N;
+    p.act = act;
+    p.beta = beta;
+    return launch_tiles<T, kDenseDz>(p, st);
+}
+
+template <typename T>
+int DenseOps<T>::dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int64_t rows, int N, int K, hipStream_t st) {
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(w), tp<T>(w2), K, K, N, N / 2};
+    p.j = {tp<T>(dz), nullptr, ld_dz, rows, N, 0};
+    p.out = static_cast<T *>(dx);
+    p.ld_out = K;
+    return launch_tiles<T, kDenseDx>(p, st);
+}
+
+template <typename T>
+int DenseOps<T>::dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, float *scratch, int64_t rows, int N, int K, hipStream_t st) {
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(x), nullptr, ld_x, K, rows, 0};
+    p.j = {tp<T>(dz), nullptr, ld_dz, N, rows, 0};
+    p.partial = scratch;
+    p.want_sums = db != nullptr;
+    p.slabs = dense_dw_slabs(rows, N, K);
+    if (int rc = launch_tiles<T, kDenseDw>(p, st)) return rc;
+    const int64_t n = (int64_t)N * K, n_db = db ? N : 0;
+    hipLaunchKernelGGL((dense_dw_sum_kernel<T>), dim3((unsigned)ceil_div<int64_t>(n + n_db, 256)), dim3(256), 0, st, scratch, p.slabs, n, n_db, static_cast<T *>(dw),
+                       static_cast<T *>(db));
+    return check_launch("dense_dw");
+}
+
+template <typename T>
+int DenseOps<T>::gated_fwd(const void *x, int64_t ld_x, const void *wg, const void *wu, const void *bg, const void *bu, void *h, int act, float beta, int64_t rows, int K,
+                           int H, hipStream_t st) {
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(wg), tp<T>(wu), K, H, K, 0};
+    p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
+    p.bias = tp<T>(bg);
+    p.bias2 = tp<T>(bu);
+    p.out = static_cast<T *>(h);
+    p.ld_out = H;
+    p.act = act;
+    p.beta = beta;
+    if (rows <= kFewRows) {
+        const dim3 grid((unsigned)ceil_div<int>(H, 16));
+        if (rows <= 16) hipLaunchKernelGGL((dense_few_kernel<T, true, 1>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((dense_few_kernel<T, true, 2>), grid, dim3(256), 0, st, p);
+        return check_launch("gated_fwd");
+    }
+    return launch_tiles<T, kGatedFwd>(p, st);
+}
+
+template <typename T>
+int DenseOps<T>::gated_bwd(const void *x, int64_t ld_x, const void *wg, const void *wu, const void *bg, const void *bu, const void *dy, int64_t ld_dy, const void *wd,
+                           void *dgu, int act, float beta, int64_t rows, int K, int H, int N, hipStream_t st) {
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(wg), tp<T>(wu), K, H, K, 0};
+    p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
+    p.i2 = {tp<T>(wd), nullptr, H, H, N, 0};
+    p.j2 = {tp<T>(dy), nullptr, ld_dy, rows, N, 0};
+    p.bias = tp<T>(bg);
+    p.bias2 = tp<T>(bu);
+    p.out = static_cast<T *>(dgu);
+    p.ld_out = 2 * (int64_t)H;
+    p.act = act;
+    p.beta = beta;
+    return launch_tiles<T, kGatedBwd>(p, st);
+}
+
+}  // namespace arcn

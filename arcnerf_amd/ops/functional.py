@@ -1187,6 +1187,190 @@ def mlp_bwd(x, weights, biases, desc, out, acts, dout, want_dx=True, n_dev=None,
 
 
 # ------------------------------------------------------------------------------------------------
+# residual feed-forward layers (csrc/norm.hip, csrc/dense.hpp): float32, bfloat16 and float16 rows
+# ------------------------------------------------------------------------------------------------
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+DENSE_ACT = {None: 0, 'none': 0, 'identity': 0, 'relu': 1, 'sigmoid': 2, 'softplus': 4, 'silu': 7, 'gelu': 8}
+
+
+def _dense_act(act, beta):
+    code = DENSE_ACT.get(act.lower() if isinstance(act, str) else act)
+    if code is None:
+        raise RuntimeError('arcnerf_amd: no activation {!r} in the dense layers (one of {})'.format(act, sorted(k for k in DENSE_ACT if k)))
+    if code == 4 and not beta > 0:
+        raise RuntimeError('arcnerf_amd: softplus needs beta > 0 (got {})'.format(beta))
+    return code
+
+
+def _ffn_rows(name, t, width=None, like=None):
+    """(2-D row operand, its row stride in elements): rows at any stride as they are (a column slice of a wider buffer), anything else
+    contiguous; checked against the width, and the device and type of `like`"""
+    if t.dim() != 2 or (width is not None and t.shape[1] != width):
+        raise RuntimeError('arcnerf_amd: {} must be (rows, {}), got {}'.format(name, 'width' if width is None else width, tuple(t.shape)))
+    if t.dtype not in _DTYPE:
+        raise RuntimeError('arcnerf_amd: {} is {}; float32, bfloat16 and float16 are taken'.format(name, t.dtype))
+    if like is not None:
+        if t.dtype != like.dtype or t.device != like.device:
+            raise RuntimeError('arcnerf_amd: {} is {} on {}, the rows are {} on {}'.format(name, t.dtype, t.device, like.dtype, like.device))
+        if t.shape[0] != like.shape[0]:
+            raise RuntimeError('arcnerf_amd: {} has {} rows, not {}'.format(name, t.shape[0], like.shape[0]))
+    if t.shape[1] < 1:
+        raise RuntimeError('arcnerf_amd: {} has no columns'.format(name))
+    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+        return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    t = t.contiguous()
+    return t, t.shape[1]
+
+
+def _ffn_param(name, t, shape, like, types=None):
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or t.device != like.device or t.dtype not in (types or (like.dtype,)):
+        raise RuntimeError('arcnerf_amd: {} must be {} {} on {}, got {} {} on {}'.format(
+            name, tuple(shape), ' / '.join(str(d) for d in (types or (like.dtype,))), like.device, tuple(t.shape), t.dtype, t.device))
+    return t.contiguous()
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _device_of(t):
+    """the launches of a call go to its tensors' device, whatever the current one is"""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=False):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the rows of x (S, C); weight / bias (C): x's type, or float32, both the same.
+    want_stats: also the (S, 2) float32 mean and 1 / sqrt(var + eps) that layer_norm_bwd takes"""
+    _req(x, weight, bias)
+    x, ld = _ffn_rows('x', x)
+    S, C = x.shape
+    wt = weight if weight is not None else bias
+    types = (x.dtype, torch.float32) if weight is None or bias is None else (weight.dtype,) if weight.dtype in (x.dtype, torch.float32) else (x.dtype,)
+    weight, bias = _ffn_param('weight', weight, (C,), x, types), _ffn_param('bias', bias, (C,), x, types)
+    y = _fresh((S, C), x.dtype, x.device)
+    stats = _fresh((S, 2), torch.float32, x.device) if want_stats else None
+    with _device_of(x):
+        N.check(N.lib().arcn_layer_norm_fwd(x.data_ptr(), ld, N.ptr(weight), N.ptr(bias), _DTYPE[x.dtype], _DTYPE[x.dtype if wt is None else wt.dtype],
+                                            float(eps), N.ptr(y), N.ptr(stats), S, C, N.stream()), 'layer_norm_fwd')
+    return (y, stats) if want_stats else y
+
+
+def layer_norm_bwd(x, dy, weight, stats, want_dx=True, want_dw=True, want_db=True, param_dtype=None):
+    """(dx, dweight, dbias) of layer_norm_fwd, None where not wanted; the parameters' gradients in weight's type (param_dtype where weight is None)"""
+    _req(x, dy, weight, stats)
+    x, ld = _ffn_rows('x', x)
+    S, C = x.shape
+    dy, ld_dy = _ffn_rows('dy', dy, C, like=x)
+    weight = _ffn_param('weight', weight, (C,), x, (x.dtype, torch.float32))
+    wt = weight.dtype if weight is not None else (param_dtype or x.dtype)
+    if tuple(stats.shape) != (S, 2) or stats.dtype != torch.float32 or stats.device != x.device:
+        raise RuntimeError('arcnerf_amd: stats must be the ({}, 2) float32 that layer_norm_fwd gave'.format(S))
+    dx = _fresh((S, C), x.dtype, x.device) if want_dx else None
+    if S == 0:
+        return dx, *(torch.zeros(C, dtype=wt, device=x.device) if want else None for want in (want_dw, want_db))
+    dw = _fresh((C,), wt, x.device) if want_dw else None
+    db = _fresh((C,), wt, x.device) if want_db else None
+    nf = int(N.lib().arcn_layer_norm_bwd_scratch_floats(S, C, _DTYPE[x.dtype])) if want_dw or want_db else 0
+    scratch = torch.empty(nf, dtype=torch.float32, device=x.device) if nf else None
+    with _device_of(x):
+        N.check(N.lib().arcn_layer_norm_bwd(x.data_ptr(), ld, dy.data_ptr(), ld_dy, N.ptr(weight), N.ptr(stats.contiguous()), _DTYPE[x.dtype], _DTYPE[wt],
+                                            N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(scratch), nf, S, C, N.stream()), 'layer_norm_bwd')
+    return dx, dw, db
+
+
+def dense_fwd(x, w, bias=None, residual=None, act=None, beta=1.0):
+    """act(x (S, K) @ w (N, K).T + bias) + residual, float32 / bfloat16 / float16 (one type for all), rounded once; act: DENSE_ACT"""
+    _req(x, w, bias, residual)
+    x, ld = _ffn_rows('x', x)
+    (S, K), Nn, code = x.shape, w.shape[0], _dense_act(act, beta)
+    w, bias = _ffn_param('weight', w, (Nn, K), x), _ffn_param('bias', bias, (Nn,), x)
+    res, ld_res = (None, 0) if residual is None else _ffn_rows('residual', residual, Nn, like=x)
+    y = _fresh((S, Nn), x.dtype, x.device)
+    with _device_of(x):
+        N.check(N.lib().arcn_dense_fwd(x.data_ptr(), ld, N.ptr(w), N.ptr(bias), None if res is None else res.data_ptr(), ld_res, N.ptr(y), _DTYPE[x.dtype],
+                                       code, float(beta), S, K, Nn, N.stream()), 'dense_fwd')
+    return y
+
+
+def dense_dz(x, w, bias, dy, act, beta=1.0):
+    """dy * act'(x @ w.T + bias), the pre-activation computed again; dy itself where there is no activation"""
+    _req(x, w, bias, dy)
+    x, ld = _ffn_rows('x', x)
+    (S, K), Nn, code = x.shape, w.shape[0], _dense_act(act, beta)
+    w, bias = _ffn_param('weight', w, (Nn, K), x), _ffn_param('bias', bias, (Nn,), x)
+    dy, ld_dy = _ffn_rows('dy', dy, Nn, like=x)
+    if code == 0:
+        return dy
+    dz = _fresh((S, Nn), x.dtype, x.device)
+    with _device_of(x):
+        N.check(N.lib().arcn_dense_dz(x.data_ptr(), ld, N.ptr(w), N.ptr(bias), dy.data_ptr(), ld_dy, N.ptr(dz), _DTYPE[x.dtype], code, float(beta), S, K, Nn,
+                                      N.stream()), 'dense_dz')
+    return dz
+
+
+def dense_dx(dz, w, w2=None):
+    """dz (S, N) @ w (N, K), or @ [w; w2] for a weight in two halves"""
+    _req(dz, w, w2)
+    dz, ld = _ffn_rows('dz', dz)
+    (S, Nn), K = dz.shape, w.shape[1]
+    rows = Nn if w2 is None else Nn // 2
+    if w2 is not None and Nn % 2:
+        raise RuntimeError('arcnerf_amd: dz of two weights has an even width, got {}'.format(Nn))
+    w, w2 = _ffn_param('weight', w, (rows, K), dz), _ffn_param('weight 2', w2, (rows, K), dz)
+    dx = _fresh((S, K), dz.dtype, dz.device)
+    with _device_of(dz):
+        N.check(N.lib().arcn_dense_dx(dz.data_ptr(), ld, N.ptr(w), N.ptr(w2), N.ptr(dx), _DTYPE[dz.dtype], S, Nn, K, N.stream()), 'dense_dx')
+    return dx
+
+
+def dense_dw(dz, x, want_db=False):
+    """(dz (S, N).T @ x (S, K), column sums of dz or None), summed over the rows in a fixed order"""
+    _req(dz, x)
+    x, ld_x = _ffn_rows('x', x)
+    dz, ld = _ffn_rows('dz', dz, like=x)
+    (S, K), Nn = x.shape, dz.shape[1]
+    dw = _fresh((Nn, K), x.dtype, x.device)
+    db = _fresh((Nn,), x.dtype, x.device) if want_db else None
+    nf = int(N.lib().arcn_dense_dw_scratch_floats(S, Nn, K))
+    scratch = torch.empty(nf, dtype=torch.float32, device=x.device)
+    with _device_of(x):
+        N.check(N.lib().arcn_dense_dw(dz.data_ptr(), ld, x.data_ptr(), ld_x, N.ptr(dw), N.ptr(db), _DTYPE[x.dtype], N.ptr(scratch), nf, S, Nn, K, N.stream()),
+                'dense_dw')
+    return dw, db
+
+
+def gated_fwd(x, w_gate, w_up, b_gate=None, b_up=None, act='silu', beta=1.0):
+    """act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up), both weights (H, K), in one pass over x"""
+    _req(x, w_gate, w_up, b_gate, b_up)
+    x, ld = _ffn_rows('x', x)
+    (S, K), H, code = x.shape, w_gate.shape[0], _dense_act(act, beta)
+    w_gate, w_up = _ffn_param('w_gate', w_gate, (H, K), x), _ffn_param('w_up', w_up, (H, K), x)
+    b_gate, b_up = _ffn_param('b_gate', b_gate, (H,), x), _ffn_param('b_up', b_up, (H,), x)
+    h = _fresh((S, H), x.dtype, x.device)
+    with _device_of(x):
+        N.check(N.lib().arcn_gated_fwd(x.data_ptr(), ld, N.ptr(w_gate), N.ptr(w_up), N.ptr(b_gate), N.ptr(b_up), N.ptr(h), _DTYPE[x.dtype], code, float(beta),
+                                       S, K, H, N.stream()), 'gated_fwd')
+    return h
+
+
+def gated_bwd(x, w_gate, w_up, b_gate, b_up, dy, w_down, act='silu', beta=1.0):
+    """(S, 2 H) = [d gate | d up], the gradients of the two pre-activations of gated_fwd for the gradient dy (S, N) of h @ w_down (N, H).T: both
+    pre-activations and dy @ w_down are computed in the kernel"""
+    _req(x, w_gate, w_up, b_gate, b_up, dy, w_down)
+    x, ld = _ffn_rows('x', x)
+    (S, K), H, Nn, code = x.shape, w_gate.shape[0], w_down.shape[0], _dense_act(act, beta)
+    w_gate, w_up = _ffn_param('w_gate', w_gate, (H, K), x), _ffn_param('w_up', w_up, (H, K), x)
+    b_gate, b_up, w_down = _ffn_param('b_gate', b_gate, (H,), x), _ffn_param('b_up', b_up, (H,), x), _ffn_param('w_down', w_down, (Nn, H), x)
+    dy, ld_dy = _ffn_rows('dy', dy, Nn, like=x)
+    dgu = _fresh((S, 2 * H), x.dtype, x.device)
+    with _device_of(x):
+        N.check(N.lib().arcn_gated_bwd(x.data_ptr(), ld, N.ptr(w_gate), N.ptr(w_up), N.ptr(b_gate), N.ptr(b_up), dy.data_ptr(), ld_dy, N.ptr(w_down), N.ptr(dgu),
+                                       _DTYPE[x.dtype], code, float(beta), S, K, H, Nn, N.stream()), 'gated_bwd')
+    return dgu
+
+
+# ------------------------------------------------------------------------------------------------
 # compositing
 # ------------------------------------------------------------------------------------------------
 def _bkg(bkg_color, R):

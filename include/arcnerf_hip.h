@@ -9,7 +9,8 @@
  *     call returns immediately.
  *   - return value: 0 = ok, ARCN_EINVAL (-1) = bad argument, ARCN_ELAUNCH (-2) = hip launch error
  *     (arcn_last_error() returns the hip error string).
- *   - fp32 everywhere ("dtype": "f32"); contiguous row-major tensors, same shapes as the reference ops.
+ *   - fp32 everywhere ("dtype": "f32"), but for the feed-forward layers at the end, which also take bf16 and f16; contiguous
+ *     row-major tensors, same shapes as the reference ops.
  *
  * Each entry point cites the reference interface it replaces (file:line relative to the ArcNerf repo).
  */
@@ -38,6 +39,14 @@ extern "C" {
 #define ARCN_ACT_SQUAREPLUS 5 /* y = (X + sqrt(X^2 + 4)) / 2 / 10 with X = 10 x; dy/dx = Y^2 / (Y^2 + 1), Y = 10 y */
 #define ARCN_ACT_SINE 6       /* y = sin(x); dy/dx = cos(x) needs the PRE-activation: elementwise ops and forward passes only - the fused
                                * MLP backward works from the post-activations it saved and refuses Sine (tiny-cuda-nn's fused MLP does too) */
+/* the activations of feed-forward blocks: taken by arcn_dense_* and arcn_gated_* alone (together with NONE, RELU, SIGMOID, SOFTPLUS) */
+#define ARCN_ACT_SILU 7 /* y = x / (1 + exp(-x)) */
+#define ARCN_ACT_GELU 8 /* y = x (1 + erf(x / sqrt 2)) / 2 */
+
+/* element types of arcn_layer_norm_*, arcn_dense_* and arcn_gated_* (every other entry point is float32) */
+#define ARCN_DTYPE_F32 0
+#define ARCN_DTYPE_BF16 1
+#define ARCN_DTYPE_F16 2
 
 const char *arcn_last_error(void);
 int arcn_version(void);
@@ -799,6 +808,48 @@ int arcn_ngp_step_tail(const arcn_mlp_desc *desc_a, float *scratch_a, int64_t w_
                        int64_t w_seg_b, int64_t n_cap, int64_t n, float *param, float *grad, float *exp_avg, float *exp_avg_sq, float *ema,
                        const int64_t *runs_host, int n_runs, float lr, float beta1, float beta2, float eps, float weight_decay,
                        float ema_decay, float grad_scale, int step, int ema_step, uint32_t *clear, int64_t clear_words, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Residual feed-forward layers of wide nets (no counterpart in the reference, whose nets are the DenseLayer stacks of
+ * arcnerf/models/base_modules/geo_rad_model/linear_network_module.py:16-335): layer norm, a dense layer with activation and residual, a
+ * gated pair of dense layers; forward and first-order backward.  dtype = ARCN_DTYPE_* is the type of every `void *` tensor of a call.
+ * Sums, statistics and activations are computed in f32, results are rounded once.  Rows (x, dy, dz, residual) may start at any element
+ * and lie ld elements apart (ld >= the width); weights, biases and outputs are contiguous.  Outputs must not overlap inputs.  The
+ * reductions over rows have a fixed order: the same call gives the same bits.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* y (n_rows, C) = (x - mean) / sqrt(var + eps) * weight + bias per row; weight / bias (C) of type w_dtype (ARCN_DTYPE_F32 or dtype), either
+ * may be NULL (ones / zeros).  stats (n_rows, 2) receives mean and 1 / sqrt(var + eps) for the backward; may be NULL. */
+int arcn_layer_norm_fwd(const void *x, int64_t ld_x, const void *weight, const void *bias, int dtype, int w_dtype, float eps, void *y,
+                        float *stats, int64_t n_rows, int C, void *stream);
+/* dx (n_rows, C), dweight and dbias (C, w_dtype); each may be NULL.  scratch: arcn_layer_norm_bwd_scratch_floats floats, needed when
+ * dweight or dbias is wanted. */
+int64_t arcn_layer_norm_bwd_scratch_floats(int64_t n_rows, int C, int dtype);
+int arcn_layer_norm_bwd(const void *x, int64_t ld_x, const void *dy, int64_t ld_dy, const void *weight, const float *stats, int dtype, int w_dtype,
+                        void *dx, void *dweight, void *dbias, float *scratch, int64_t scratch_floats, int64_t n_rows, int C, void *stream);
+
+/* y (n_rows, N) = act(x (n_rows, K) w (N, K)^T + bias) + residual; bias and residual may be NULL.  act = ARCN_ACT_NONE, _RELU, _SIGMOID,
+ * _SOFTPLUS (beta > 0; identity from beta z > 20), _SILU, _GELU.  f32 products are accumulated from three-way bf16 splits of the operands
+ * (f32 accuracy; infinities and NaN give NaN). */
+int arcn_dense_fwd(const void *x, int64_t ld_x, const void *w, const void *bias, const void *residual, int64_t ld_res, void *y, int dtype, int act,
+                   float beta, int64_t n_rows, int K, int N, void *stream);
+/* dz (n_rows, N) = dy act'(x w^T + bias): the gradient of the pre-activation, which is computed again from x (nothing was saved) */
+int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, int dtype, int act, float beta,
+                  int64_t n_rows, int K, int N, void *stream);
+/* dx (n_rows, K) = dz (n_rows, N) w (N, K).  w2 not NULL (N even): the weight's first N / 2 rows are w (N / 2, K), the others w2. */
+int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int dtype, int64_t n_rows, int N, int K, void *stream);
+/* dw (N, K) = dz^T x and, unless db is NULL, db (N) = the column sums of dz.  scratch: arcn_dense_dw_scratch_floats floats. */
+int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K);
+int arcn_dense_dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, int dtype, float *scratch, int64_t scratch_floats,
+                  int64_t n_rows, int N, int K, void *stream);
+/* h (n_rows, H) = act(x w_gate^T + b_gate) * (x w_up^T + b_up); w_gate and w_up (H, K), biases (H) or NULL */
+int arcn_gated_fwd(const void *x, int64_t ld_x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, void *h, int dtype, int act,
+                   float beta, int64_t n_rows, int K, int H, void *stream);
+/* The gated block's inner gradients for y = h w_down^T (w_down (N, H), dy (n_rows, N)): with dh = dy w_down, g = x w_gate^T + b_gate and
+ * u = x w_up^T + b_up (computed again, in registers), dgu (n_rows, 2 H) = [dh u act'(g) | dh act(g)].  What is left are arcn_dense_dx(dgu,
+ * w_gate, w_up) and arcn_dense_dw(dgu, x), whose (2 H, K) result is both weights' gradients, and arcn_dense_dw(dy, h). */
+int arcn_gated_bwd(const void *x, int64_t ld_x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, const void *dy, int64_t ld_dy,
+                   const void *w_down, void *dgu, int dtype, int act, float beta, int64_t n_rows, int K, int H, int N, void *stream);
 
 #ifdef __cplusplus
 }
