@@ -41,16 +41,16 @@ ARCN_EXPORT int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, cons
     return ARCN_DENSE_DISPATCH(dx(dz, ld_dz, w, w2, dx, n_rows, N, K, as_stream(stream)));
 }
 
-ARCN_EXPORT int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K) {
-    if (!dense_sizes(n_rows, K, N)) return 0;
-    return (int64_t)dense_dw_slabs(n_rows, N, K) * ((int64_t)N * K + N);
+ARCN_EXPORT int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K, int dtype) {
+    if (!dense_sizes(n_rows, K, N) || !dense_type(dtype)) return 0;
+    return (int64_t)dense_dw_slabs(dtype == ARCN_DTYPE_F32 ? 4 : 2, n_rows, N, K) * ((int64_t)N * K + N);
 }
 
 ARCN_EXPORT int arcn_dense_dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, int dtype, float *scratch, int64_t scratch_floats,
                               int64_t n_rows, int N, int K, void *stream) {
     if (!dense_type(dtype) || !dense_sizes(n_rows, K, N)) return einval("dense_dw: unsupported type or size");
     if (!dw || !scratch || (n_rows > 0 && (!dz || !x || ld_dz < N || ld_x < K))) return einval("dense_dw: missing / invalid argument");
-    if (scratch_floats < arcn_dense_dw_scratch_floats(n_rows, N, K)) return einval("dense_dw: scratch smaller than arcn_dense_dw_scratch_floats");
+    if (scratch_floats < arcn_dense_dw_scratch_floats(n_rows, N, K, dtype)) return einval("dense_dw: scratch smaller than arcn_dense_dw_scratch_floats");
     return ARCN_DENSE_DISPATCH(dw(dz, ld_dz, x, ld_x, dw, db, scratch, n_rows, N, K, as_stream(stream)));
 }
 

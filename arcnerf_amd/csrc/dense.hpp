@@ -17,13 +17,15 @@
 // lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  416 TFLOP/s of f32-accurate products against 157
 // on the f32 MFMA.  Infinities and NaN in such an operand give NaN.
 //
-// A tile's I rows are dealt to MFMA tiles in pairs: MFMA row 4 g + r of tile m is feature 32 (m / 2) + 8 g + 4 (m % 2) + r, so that a
-// lane's accumulators of two tiles are 8 CONSECUTIVE features of one row: residual, gradient and result move as 16 bytes per lane.
+// A lane's accumulators of one MFMA tile are 4 consecutive features of a row; the tiles are taken in pairs and lane rows 1 and 3 of the
+// first are swapped with lane rows 0 and 2 of the second (v_permlane16_swap_b32), which leaves 8 CONSECUTIVE features of one row in each
+// lane: residual, gradient and result move as 16 bytes per lane, 64 bytes per row and instruction.
 #pragma once
 
 #include <type_traits>
 
 #include "elem.hpp"
+#include "partials.hpp"
 
 #pragma clang fp contract(fast)
 
@@ -43,40 +45,75 @@ __device__ __forceinline__ float exp_hw(float x) {
     return fmaf(e * 0.693147181f, lo, e);
 }
 
-template <bool SLOPE>
-__device__ __forceinline__ float act_eval(float z, int act, float beta, float &slope) {
-    switch (act) {
-    case ARCN_ACT_RELU:
+// FAST (16-bit results): the exponential without that correction (x 2^-24 of itself, 2^-18 at most where the result counts) and the error
+// function by Abramowitz and Stegun 7.1.26 (1.5e-7), which shares its exponential with the slope: a third of the instructions of an epilogue
+// that is all of a wide tile's vector work
+template <int ACT, bool SLOPE, bool FAST>
+__device__ __forceinline__ float act_eval(float z, float beta, float inv_beta, float &slope) {
+    if constexpr (ACT == ARCN_ACT_RELU) {
         if (SLOPE) slope = z <= 0.f ? 0.f : 1.f;
         return z <= 0.f ? 0.f : z;      // (a NaN stays one)
-    case ARCN_ACT_SIGMOID:
-    case ARCN_ACT_SILU: {
-        const float e = exp_hw(-fabsf(z)), q = __builtin_amdgcn_rcpf(1.f + e);
-        const float s = z >= 0.f ? q : e * q;
-        if (act == ARCN_ACT_SIGMOID) {
-            if (SLOPE) slope = e * q * q;
-            return s;
+    } else if constexpr (FAST && (ACT == ARCN_ACT_SIGMOID || ACT == ARCN_ACT_SILU)) {
+        const float q = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+        if constexpr (ACT == ARCN_ACT_SIGMOID) {
+            if (SLOPE) slope = q * (1.f - q);
+            return q;
+        } else {
+            if (SLOPE) slope = q * fmaf(z, 1.f - q, 1.f);
+            return z * q;
         }
-        const float one_minus = z >= 0.f ? e * q : q;
-        if (SLOPE) slope = s * (1.f + z * one_minus);
-        return z * s;
-    }
-    case ARCN_ACT_SOFTPLUS: {
+    } else if constexpr (ACT == ARCN_ACT_SIGMOID || ACT == ARCN_ACT_SILU) {
+        const float e = exp_hw(-fabsf(z)), q = __builtin_amdgcn_rcpf(1.f + e), eq = e * q;
+        const bool up = z >= 0.f;
+        const float s = up ? q : eq;
+        if constexpr (ACT == ARCN_ACT_SIGMOID) {
+            if (SLOPE) slope = eq * q;
+            return s;
+        } else {
+            if (SLOPE) slope = s * (1.f + z * (up ? eq : q));
+            return z * s;
+        }
+    } else if constexpr (ACT == ARCN_ACT_SOFTPLUS) {
         // log1p(t) = log(u) t / (u - 1) with u = fl(1 + t): the rounding of 1 + t cancels
         const float bz = beta * z;
-        const float t = exp_hw(-fabsf(bz)), u = 1.f + t, q = __builtin_amdgcn_rcpf(u);
-        if (SLOPE) slope = bz > 20.f ? 1.f : (bz >= 0.f ? q : t * q);
-        const float l = u == 1.f ? t : __logf(u) * (t / (u - 1.f));
-        return bz > 20.f ? z : (fmaxf(bz, 0.f) + l) / beta;
-    }
-    case ARCN_ACT_GELU: {
+        const float t = FAST ? __builtin_amdgcn_exp2f(fabsf(bz) * -1.44269504f) : exp_hw(-fabsf(bz)), u = 1.f + t;
+        if (SLOPE) {
+            const float q = __builtin_amdgcn_rcpf(u);
+            slope = bz > 20.f ? 1.f : (bz >= 0.f ? q : t * q);
+        }
+        const float l = u == 1.f ? t : __logf(u) * (t * __builtin_amdgcn_rcpf(u - 1.f));
+        return bz > 20.f ? z : (fmaxf(bz, 0.f) + l) * inv_beta;
+    } else if constexpr (FAST && ACT == ARCN_ACT_GELU) {
+        const float e = __builtin_amdgcn_exp2f(z * z * -0.721347520f);                                   // e^(-z^2 / 2)
+        const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.231641888f, 1.f));                        // 1 / (1 + p |z| / sqrt 2)
+        float q = fmaf(t, 1.061405429f, -1.453152027f);
+        q = fmaf(t, q, 1.421413741f);
+        q = fmaf(t, q, -0.284496736f);
+        q = fmaf(t, q, 0.254829592f) * t * e * 0.5f;                                                     // half of erfc(|z| / sqrt 2)
+        const float cdf = z > 0.f ? 1.f - q : q;
+        if (SLOPE) slope = fmaf(z * 0.398942280f, e, cdf);
+        return z * cdf;
+    } else if constexpr (ACT == ARCN_ACT_GELU) {
         const float cdf = 0.5f * (1.f + erff(z * 0.707106781f));
         if (SLOPE) slope = fmaf(z * 0.398942280f, exp_hw(-0.5f * z * z), cdf);
         return z * cdf;
-    }
-    default:
+    } else {
         if (SLOPE) slope = 1.f;
         return z;
+    }
+}
+
+// f(activation as a compile-time number): the choice is made once per tile, not once per element (64 copies of a switch over all the
+// activations do not fit the instruction cache: a 256-wide bf16 layer of 262144 rows took 249 us with them, 135 without)
+template <typename Fn>
+__device__ __forceinline__ void with_act(int act, Fn &&f) {
+    switch (act) {
+    case ARCN_ACT_RELU: f(std::integral_constant<int, ARCN_ACT_RELU>{}); break;
+    case ARCN_ACT_SIGMOID: f(std::integral_constant<int, ARCN_ACT_SIGMOID>{}); break;
+    case ARCN_ACT_SOFTPLUS: f(std::integral_constant<int, ARCN_ACT_SOFTPLUS>{}); break;
+    case ARCN_ACT_SILU: f(std::integral_constant<int, ARCN_ACT_SILU>{}); break;
+    case ARCN_ACT_GELU: f(std::integral_constant<int, ARCN_ACT_GELU>{}); break;
+    default: f(std::integral_constant<int, ARCN_ACT_NONE>{}); break;
     }
 }
 
@@ -105,13 +142,16 @@ struct Mma<float> {
     static __device__ __forceinline__ f4v one(s8v a, s8v b, f4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c) {   // smallest terms first
-        c = one(a[1], b[1], c);
-        c = one(a[0], b[2], c);
-        c = one(a[2], b[0], c);
-        c = one(a[0], b[1], c);
-        c = one(a[1], b[0], c);
-        return one(a[0], b[0], c);
+    // the six terms of 32 reduction elements among themselves, smallest first, then ONE addition (rounded to nearest) to the running sum:
+    // six accumulations straight into it would round at its size six times
+    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c) {
+        f4v t = {0.f, 0.f, 0.f, 0.f};
+        t = one(a[1], b[1], t);
+        t = one(a[0], b[2], t);
+        t = one(a[2], b[0], t);
+        t = one(a[0], b[1], t);
+        t = one(a[1], b[0], t);
+        return c + one(a[0], b[0], t);
     }
     static constexpr short kOne = 0x3f80;
 };
@@ -176,27 +216,34 @@ struct Operand {
     int64_t split;
 };
 
-// R: output indices of the tile.  PAIR: the I operand (MFMA tiles in pairs), else the J operand.  GATED: rows alternate between two matrices.
-template <typename T, int R, int THREADS, bool TR, bool PAIR, bool GATED>
+// R: output indices of the tile.  GATED: its rows alternate, in groups of 32, between two matrices.
+template <typename T, int R, int THREADS, bool TR, bool GATED>
 struct Tile {
     static constexpr int BK = Mma<T>::BK, P = Mma<T>::P;
-    static constexpr int CHUNKS = R * BK / 8, N = (CHUNKS + THREADS - 1) / THREADS;
-    static constexpr int kElems = P * R * BK;   // of one LDS buffer
+    static constexpr int CHUNKS = R * BK / 8, N = (CHUNKS + THREADS - 1) / THREADS;   // chunk: 8 elements
+    static constexpr int PER_ROW = TR ? R / 8 : BK / 8;                              // chunks of an LDS row (TR: a reduction row)
+    static constexpr int kElems = P * R * BK;                                        // of one LDS buffer
     Raw8<T> raw[N];
 
-    // place of chunk c (8 elements) of tile row `row` in a plane, in elements.  The swizzles spread what one read instruction's lanes
-    // touch over all banks: 8 lanes of a 16-byte read over eight 16-byte places, 16 lanes of an 8-byte transposing read (4 rows) over
-    // sixteen 8-byte ones.
+    // chunk c of LDS row `row` is kept at chunk c ^ swizzle(row): the 8 lanes that one cycle of a 16-byte read serves, and the 16 of an
+    // 8-byte transposing read (4 rows), fall on different banks.  (Its own inverse.  A row of 4 chunks shares its 128 bytes with the next.)
     static __device__ __forceinline__ int place(int row, int c) {
-        if (!TR) {
-            const int q = row * (BK / 8) + c, line = q >> 3;
-            const int s = BK == 64 ? (PAIR ? ((line & 3) | ((line >> 1) & 4)) : (line & 7)) : (PAIR ? ((line & 1) | ((line >> 1) & 2)) : (line & 3));
-            return 8 * (q ^ s);
-        }
-        if (R < 64) return 8 * (row * (R / 8) + c);
-        return 8 * (row * (R / 8) + (c ^ (PAIR ? ((row & 1) << 2) : ((row & 3) << 1))));
+        if (TR) return 8 * (row * PER_ROW + (PER_ROW >= 8 ? c ^ ((row & 3) << 1) : c));
+        if (BK == 64) return 8 * (row * PER_ROW + (c ^ (row & 7)));
+        return 8 * ((row * PER_ROW + c) ^ ((row >> 1) & 3));
     }
-    static __device__ __forceinline__ bool halves_swapped(int row) { return TR && PAIR && R >= 64 && (row & 2); }
+
+    // address of chunk c of LDS row `row` when the reduction stands at k0
+    static __device__ __forceinline__ const T *source(const Operand<T> &op, int64_t out0, int64_t k0, int row, int c) {
+        if (!TR) {
+            // (a row behind the operand's last one is computed and dropped: it reads the last one)
+            int64_t out = out0 + (GATED ? ((row >> 6) * 32 + (row & 31)) : row);
+            out = out < op.n_out ? out : op.n_out - 1;
+            return (GATED && (row & 32) ? op.b : op.a) + out * op.ld + k0 + 8 * c;
+        }
+        const int64_t r = k0 + row;
+        return (op.b && r >= op.split ? op.b + (r - op.split) * op.ld : op.a + r * op.ld) + out0 + 8 * c;
+    }
 
     __device__ __forceinline__ void fetch(const Operand<T> &op, int64_t out0, int64_t k0, int64_t k_end, int tid) {
         const bool full = k0 + BK <= k_end && (!TR || out0 + R <= op.n_out);
@@ -204,19 +251,10 @@ struct Tile {
         for (int n = 0; n < N; ++n) {
             const int q = tid + n * THREADS;
             if (CHUNKS % THREADS && q >= CHUNKS) break;
-            if (!TR) {
-                const int row = q / (BK / 8), c = q % (BK / 8);
-                // (a row behind the operand's last one is computed and dropped: it reads the last one)
-                int64_t out = out0 + (GATED ? ((row >> 6) * 32 + (row & 31)) : row);
-                out = out < op.n_out ? out : op.n_out - 1;
-                const T *p = (GATED && (row & 32) ? op.b : op.a) + out * op.ld + k0 + 8 * c;
-                raw[n] = full ? load8<T>(p) : load8<T>(p, k_end - (k0 + 8 * c));
-            } else {
-                const int row = q / (R / 8), c = q % (R / 8);
-                const int64_t r = k0 + row, out = out0 + 8 * c;
-                const T *p = (op.b && r >= op.split ? op.b + (r - op.split) * op.ld : op.a + r * op.ld) + out;
-                raw[n] = full ? load8<T>(p) : load8<T>(p, r < k_end ? op.n_out - out : 0);
-            }
+            const int row = q / PER_ROW, c = q % PER_ROW;
+            const T *p = source(op, out0, k0, row, c);
+            if (full) raw[n] = load8<T>(p);
+            else raw[n] = load8<T>(p, TR ? (k0 + row < k_end ? op.n_out - (out0 + 8 * c) : 0) : k_end - (k0 + 8 * c));
         }
     }
 
@@ -225,42 +263,47 @@ struct Tile {
         for (int n = 0; n < N; ++n) {
             const int q = tid + n * THREADS;
             if (CHUNKS % THREADS && q >= CHUNKS) break;
-            const int row = TR ? q / (R / 8) : q / (BK / 8), c = TR ? q % (R / 8) : q % (BK / 8);
             s8v pl[P];
             planes8<T>(raw[n], pl);
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                u4v v = __builtin_bit_cast(u4v, pl[p]);
-                if (TR && PAIR && R >= 64) {
-                    const bool sw = halves_swapped(row);
-                    v = u4v{sw ? v[2] : v[0], sw ? v[3] : v[1], sw ? v[0] : v[2], sw ? v[1] : v[3]};
-                }
-                *reinterpret_cast<u4v *>(lds + p * R * BK + place(row, c)) = v;
-            }
+            for (int p = 0; p < P; ++p) *reinterpret_cast<s8v *>(lds + p * R * BK + place(q / PER_ROW, q % PER_ROW)) = pl[p];
         }
     }
 
-    // fragment of MFMA tile m (from tile row / column `base`) at reduction step kk (32 elements): lane l holds output index l % 16 (as
-    // dealt), reduction elements 8 (l / 16) .. + 7
+    // memory to LDS without registers (16-bit types, 16-byte aligned rows, whole steps of the reduction): a wave's 64 chunks land in
+    // consecutive places, so the lane whose place it is asks for the chunk that belongs there
+    static __device__ __forceinline__ void copy(const Operand<T> &op, int64_t out0, int64_t k0, short *lds, int tid) {
+        const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (CHUNKS % THREADS && n * THREADS + wave0 >= CHUNKS) break;
+            const int q = tid + n * THREADS, row = q / PER_ROW;
+            int c = (place(row, q % PER_ROW) >> 3) - row * PER_ROW;
+            int64_t o0 = out0;
+            if (TR && o0 + 8 * c + 8 > op.n_out) o0 = op.n_out - 8 - 8 * c;   // (dropped outputs read the last ones)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)source(op, o0, k0, row, c),
+                                             (__attribute__((address_space(3))) void *)(lds + 8 * (n * THREADS + wave0)), 16, 0, 0);
+        }
+    }
+
+    // fragment of MFMA tile m (from tile row / column `base`) at reduction step kk (32 elements): lane l holds output index l % 16,
+    // reduction elements 8 (l / 16) .. + 7
     static __device__ __forceinline__ void frag(const short *lds, int base, int m, int kk, int lane, s8v *f) {
         const int o = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const short *pl = lds + p * R * BK;
             if (!TR) {
-                const int row = base + (PAIR ? 32 * (m >> 1) + 8 * (o >> 2) + 4 * (m & 1) + (o & 3) : 16 * m + o);
-                f[p] = *reinterpret_cast<const s8v *>(pl + place(row, 4 * kk + g));
+                f[p] = *reinterpret_cast<const s8v *>(pl + place(base + 16 * m + o, 4 * kk + g));
             } else {
                 // lane o of a group of 16 asks for 4 output indices (quad o % 4) of reduction row o / 4 and receives 4 reduction rows of
                 // output index o
-                const int col = base + (PAIR ? 32 * (m >> 1) + 8 * (o & 3) + 4 * (m & 1) : 16 * m + 4 * (o & 3));
+                const int col = base + 16 * m + 4 * (o & 3);
                 s4v h[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = 32 * kk + 8 * g + 4 * e + (o >> 2);
-                    const int at = place(row, col >> 3) + ((col & 4) ^ (halves_swapped(row) ? 4 : 0));
-                    h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)(pl + at));
-                }
+                for (int e = 0; e < 2; ++e)
+                    h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s4v *)(pl + place(32 * kk + 8 * g + 4 * e + (o >> 2), col >> 3) + (col & 4)));
                 f[p] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
             }
         }
@@ -279,7 +322,7 @@ struct DenseArgs {
     float *partial;          // kDenseDw: [slab][n_j * n_i (+ n_j column sums of j)]
     int want_sums;
     int act;
-    float beta;
+    float beta, inv_beta;
     int64_t tiles_i, tiles;  // tiles: of the whole product (times the slabs)
     int slabs;
 };
@@ -291,7 +334,8 @@ __device__ __forceinline__ int64_t xcd_tile() {
     return (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
 }
 
-template <typename T, int MODE, int WI, int WJ, int MI, int NJ>
+// ASYNC: operands straight from memory to LDS (Tile::copy; launch_tiles checks what it needs)
+template <typename T, int MODE, int WI, int WJ, int MI, int NJ, bool ASYNC>
 __global__ void __launch_bounds__(64 * WI *WJ, 2)
 dense_kernel(const DenseArgs<T> p) {
     constexpr int THREADS = 64 * WI * WJ, BI = 16 * MI * WI, BJ = 16 * NJ * WJ;
@@ -299,9 +343,9 @@ dense_kernel(const DenseArgs<T> p) {
     constexpr bool GATED = MODE == kGatedFwd || MODE == kGatedBwd;
     constexpr bool I_TR = MODE == kDenseDx || MODE == kDenseDw, J_TR = MODE == kDenseDw;
     constexpr int OUT_I = GATED ? BI / 2 : BI;      // features per tile
-    typedef Tile<T, BI, THREADS, I_TR, true, GATED> TI;
-    typedef Tile<T, BJ, THREADS, J_TR, false, false> TJ;
-    typedef Tile<T, BI / 2, THREADS, true, true, false> TI2;
+    typedef Tile<T, BI, THREADS, I_TR, GATED> TI;
+    typedef Tile<T, BJ, THREADS, J_TR, false> TJ;
+    typedef Tile<T, BI / 2, THREADS, true, false> TI2;
     constexpr int BUF = TI::kElems + TJ::kElems;
     __shared__ __attribute__((aligned(16))) short lds[NBUF * BUF];
 
@@ -331,25 +375,49 @@ dense_kernel(const DenseArgs<T> p) {
     for (int n = 0; n < (MODE == kDenseDw ? NJ : 1); ++n) sums[n] = f4v{0.f, 0.f, 0.f, 0.f};
     const bool my_sums = MODE == kDenseDw && p.want_sums && i0 == 0 && wi == 0;   // wave-uniform
 
-    auto step = [&](auto &ti, auto &tj, const short *buf, auto &c, bool add_sums) {
+    // after the swap a lane holds 8 features of a pair of tiles from 32 pr + f8, row o
+    const int g = lane >> 4, o = lane & 15, f8 = 16 * (g & 1) + 8 * (g >> 1);
+    // residual (or dy) of the lane's results.  16-bit types with registers to spare fetch it in front of the product, which hides the
+    // latency; else the registers are free only behind it
+    constexpr bool RES = MODE == kDenseFwd || MODE == kDenseDz;
+    constexpr bool RES_EARLY = RES && sizeof(T) == 2 && MI * NJ <= 16;
+    Raw8<T> res[RES ? MI / 2 : 1][RES ? NJ : 1];
+    const bool inner = i0 + OUT_I <= p.i.n_out && j0 + BJ <= p.j.n_out;    // a whole tile
+    auto fetch_res = [&]() {
+        if constexpr (RES) {
+#pragma unroll
+            for (int pr = 0; pr < MI / 2; ++pr)
+#pragma unroll
+                for (int n = 0; n < NJ; ++n) {
+                    const int64_t i = i0 + wi * 16 * MI + 32 * pr + f8, j = j0 + (wj * NJ + n) * 16 + o;
+                    const T *src = p.res + j * p.ld_res + i;
+                    if (inner) res[pr][n] = load8<T>(src);
+                    else res[pr][n] = load8<T>(src, j < p.j.n_out ? p.i.n_out - i : 0);
+                }
+        }
+    };
+    if (RES_EARLY && p.res) fetch_res();
+
+    auto step = [&](auto &ti, auto &tj, const short *buf, auto &c) {
         typedef std::remove_reference_t<decltype(ti)> Ti;
         typedef std::remove_reference_t<decltype(tj)> Tj;
         constexpr int M = sizeof(c) / sizeof(c[0]);
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
-            s8v a[M][P], b[NJ][P];
-#pragma unroll
-            for (int m = 0; m < M; ++m) Ti::frag(buf, wi * 16 * M, m, kk, lane, a[m]);
+            s8v b[NJ][P];
 #pragma unroll
             for (int n = 0; n < NJ; ++n) Tj::frag(buf + TI::kElems, wj * 16 * NJ, n, kk, lane, b[n]);
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+            for (int m = 0; m < M; ++m) {
+                s8v a[P];
+                Ti::frag(buf, wi * 16 * M, m, kk, lane, a);
 #pragma unroll
-                for (int n = 0; n < NJ; ++n) c[m][n] = Mma<T>::mma(a[m], b[n], c[m][n]);
-            if (MODE == kDenseDw && add_sums) {
-                const short o = Mma<T>::kOne;
+                for (int n = 0; n < NJ; ++n) c[m][n] = Mma<T>::mma(a, b[n], c[m][n]);
+            }
+            if (MODE == kDenseDw && my_sums) {
+                const short one = Mma<T>::kOne;
                 s8v ones[P] = {};
-                ones[0] = s8v{o, o, o, o, o, o, o, o};
+                ones[0] = s8v{one, one, one, one, one, one, one, one};
 #pragma unroll
                 for (int n = 0; n < NJ; ++n) sums[n] = Mma<T>::mma(ones, b[n], sums[n]);
             }
@@ -357,30 +425,13 @@ dense_kernel(const DenseArgs<T> p) {
     };
     auto product = [&](auto &ti, auto &tj, const Operand<T> &oi, const Operand<T> &oj, auto &c) {
         const int64_t n_steps = k_lo < k_hi ? (k_hi - k_lo + BK - 1) / BK : 0;
-        if (n_steps > 0) {
-            ti.fetch(oi, i0, k_lo, k_hi, tid);
-            tj.fetch(oj, j0, k_lo, k_hi, tid);
-        }
-        if (NBUF == 2 && n_steps > 0) {
-            ti.stash(lds, tid);
-            tj.stash(lds + TI::kElems, tid);
-            __syncthreads();
-        }
-        for (int64_t s = 0; s < n_steps; ++s) {
-            const int64_t k = k_lo + (s + 1) * BK;
-            if (NBUF == 2) {
-                short *buf = lds + (s & 1) * BUF, *next = lds + ((s & 1) ^ 1) * BUF;
-                if (s + 1 < n_steps) {
-                    ti.fetch(oi, i0, k, k_hi, tid);
-                    tj.fetch(oj, j0, k, k_hi, tid);
-                }
-                step(ti, tj, buf, c, my_sums);
-                if (s + 1 < n_steps) {
-                    ti.stash(next, tid);   // last read one step ago, behind the barrier below
-                    tj.stash(next + TI::kElems, tid);
-                }
-                __syncthreads();
-            } else {
+        if constexpr (NBUF == 1) {
+            if (n_steps > 0) {
+                ti.fetch(oi, i0, k_lo, k_hi, tid);
+                tj.fetch(oj, j0, k_lo, k_hi, tid);
+            }
+            for (int64_t s = 0; s < n_steps; ++s) {
+                const int64_t k = k_lo + (s + 1) * BK;
                 ti.stash(lds, tid);
                 tj.stash(lds + TI::kElems, tid);
                 __syncthreads();
@@ -388,8 +439,57 @@ dense_kernel(const DenseArgs<T> p) {
                     ti.fetch(oi, i0, k, k_hi, tid);
                     tj.fetch(oj, j0, k, k_hi, tid);
                 }
-                step(ti, tj, lds, c, my_sums);
+                step(ti, tj, lds, c);
                 __syncthreads();
+            }
+        } else {
+            // step s + 1 is on its way to the other buffer while step s is computed; a buffer is written again behind the barrier that
+            // follows its last read.  A last partial step goes through registers, where what lies behind the end is made zero.
+            auto through_regs = [&](int64_t s) {
+                ti.fetch(oi, i0, k_lo + s * BK, k_hi, tid);
+                tj.fetch(oj, j0, k_lo + s * BK, k_hi, tid);
+            };
+            auto put = [&](int64_t s) {
+                ti.stash(lds + (s & 1) * BUF, tid);
+                tj.stash(lds + (s & 1) * BUF + TI::kElems, tid);
+                __syncthreads();
+            };
+            if constexpr (ASYNC) {
+                auto copy = [&](int64_t s) {
+                    ti.copy(oi, i0, k_lo + s * BK, lds + (s & 1) * BUF, tid);
+                    tj.copy(oj, j0, k_lo + s * BK, lds + (s & 1) * BUF + TI::kElems, tid);
+                };
+                auto landed = [&]() {
+                    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+                    __syncthreads();
+                };
+                const int64_t whole = k_lo < k_hi ? (k_hi - k_lo) / BK : 0;
+                if (whole > 0) {
+                    copy(0);
+                    landed();
+                }
+                for (int64_t s = 0; s < whole; ++s) {
+                    if (s + 1 < whole) copy(s + 1);
+                    step(ti, tj, lds + (s & 1) * BUF, c);
+                    landed();
+                }
+                if (whole < n_steps) {
+                    through_regs(whole);
+                    put(whole);
+                    step(ti, tj, lds + (whole & 1) * BUF, c);
+                    __syncthreads();
+                }
+            } else {
+                if (n_steps > 0) {
+                    through_regs(0);
+                    put(0);
+                }
+                for (int64_t s = 0; s < n_steps; ++s) {
+                    if (s + 1 < n_steps) through_regs(s + 1);
+                    step(ti, tj, lds + (s & 1) * BUF, c);
+                    if (s + 1 < n_steps) put(s + 1);
+                    else __syncthreads();
+                }
             }
         }
     };
@@ -410,13 +510,14 @@ dense_kernel(const DenseArgs<T> p) {
         product(ti, tj, p.i2, p.j2, acc2);
     }
 
-    // ---- epilogue: lane (g, o) holds features 8 g .. 8 g + 7 of a pair of tiles, row o -------------------------------------------------
-    const int g = lane >> 4, o = lane & 15;
+    // ---- epilogue -----------------------------------------------------------------------------------------------------------------------
     auto pair8 = [&](auto &c, int pr, int n, float *v) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            v[r] = c[2 * pr][n][r];
-            v[4 + r] = c[2 * pr + 1][n][r];
+            const auto sw = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, (float)c[2 * pr][n][r]),
+                                                             __builtin_bit_cast(uint32_t, (float)c[2 * pr + 1][n][r]), false, false);
+            v[r] = __builtin_bit_cast(float, (uint32_t)sw[0]);
+            v[4 + r] = __builtin_bit_cast(float, (uint32_t)sw[1]);
         }
     };
     auto bias8 = [&](const T *b, int64_t i, float *v) {
@@ -429,100 +530,86 @@ dense_kernel(const DenseArgs<T> p) {
 #pragma unroll
         for (int n = 0; n < NJ; ++n) {
             const int64_t j = j0 + (wj * NJ + n) * 16 + o;
-            if (j >= p.j.n_out) continue;
 #pragma unroll
             for (int pr = 0; pr < MI / 2; ++pr) {
-                const int64_t i = i0 + wi * 16 * MI + 32 * pr + 8 * g;
+                const int64_t i = i0 + wi * 16 * MI + 32 * pr + f8;
                 float v[8];
                 pair8(acc, pr, n, v);
-                store8<float>(part + j * p.i.n_out + i, v, p.i.n_out - i);
+                if (j < p.j.n_out) store8<float>(part + j * p.i.n_out + i, v, p.i.n_out - i);
             }
-            if (my_sums && g == 0) part[p.i.n_out * p.j.n_out + j] = sums[n][0];
+            if (my_sums && g == 0 && j < p.j.n_out) part[p.i.n_out * p.j.n_out + j] = sums[n][0];
         }
     } else if constexpr (GATED) {
+        with_act(p.act, [&](auto A) {
 #pragma unroll
         for (int pr = 0; pr < MI / 4; ++pr) {
-            const int64_t i = i0 + wi * 8 * MI + 32 * pr + 8 * g;
-            if (i >= p.i.n_out) continue;
+            const int64_t i = i0 + wi * 8 * MI + 32 * pr + f8;
             float bg[8], bu[8];
             bias8(p.bias, i, bg);
             bias8(p.bias2, i, bu);
 #pragma unroll
             for (int n = 0; n < NJ; ++n) {
                 const int64_t j = j0 + (wj * NJ + n) * 16 + o;
-                if (j >= p.j.n_out) continue;
+                const int64_t left = j < p.j.n_out ? p.i.n_out - i : 0;
                 float gv[8], uv[8];
-                pair8(acc, 2 * pr, n, gv);
+                pair8(acc, 2 * pr, n, gv);      // (every lane takes part in the swaps)
                 pair8(acc, 2 * pr + 1, n, uv);
                 T *dst = p.out + j * p.ld_out + i;
                 if constexpr (MODE == kGatedFwd) {
                     float slope;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) gv[e] = act_eval<false>(gv[e] + bg[e], p.act, p.beta, slope) * (uv[e] + bu[e]);
-                    store8<T>(dst, gv, p.i.n_out - i);
+                    for (int e = 0; e < 8; ++e) gv[e] = act_eval<A(), false, sizeof(T) == 2>(gv[e] + bg[e], p.beta, p.inv_beta, slope) * (uv[e] + bu[e]);
+                    store8<T>(dst, gv, left);
                 } else {
                     float dh[8];
                     pair8(acc2, pr, n, dh);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float slope;
-                        const float a = act_eval<true>(gv[e] + bg[e], p.act, p.beta, slope);
+                        const float a = act_eval<A(), true, sizeof(T) == 2>(gv[e] + bg[e], p.beta, p.inv_beta, slope);
                         gv[e] = dh[e] * (uv[e] + bu[e]) * slope;
                         uv[e] = dh[e] * a;
                     }
-                    store8<T>(dst, gv, p.i.n_out - i);
-                    store8<T>(dst + p.i.n_out, uv, p.i.n_out - i);   // du behind dg in a row of 2 H
+                    store8<T>(dst, gv, left);
+                    store8<T>(dst + p.i.n_out, uv, left);   // du behind dg in a row of 2 H
                 }
             }
         }
+        });
     } else {
+        if (RES && !RES_EARLY && p.res) fetch_res();
+        with_act(RES ? p.act : ARCN_ACT_NONE, [&](auto A) {
 #pragma unroll
         for (int pr = 0; pr < MI / 2; ++pr) {
-            const int64_t i = i0 + wi * 16 * MI + 32 * pr + 8 * g;
-            if (i >= p.i.n_out) continue;
+            const int64_t i = i0 + wi * 16 * MI + 32 * pr + f8;
             float b[8];
             bias8(MODE == kDenseDx ? nullptr : p.bias, i, b);
 #pragma unroll
             for (int n = 0; n < NJ; ++n) {
                 const int64_t j = j0 + (wj * NJ + n) * 16 + o;
-                if (j >= p.j.n_out) continue;
                 float v[8];
                 pair8(acc, pr, n, v);
-                if (MODE != kDenseDx) {
-                    float r[8] = {};
-                    if (p.res) unpack8<T>(load8<T>(p.res + j * p.ld_res + i, p.i.n_out - i), r);
+                if constexpr (RES) {
+                    float r[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[e] = 0.f;
+                    if (p.res) unpack8<T>(res[pr][n], r);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float slope = 1.f;
                         if (MODE == kDenseFwd) {
-                            v[e] = act_eval<false>(v[e] + b[e], p.act, p.beta, slope) + r[e];
+                            v[e] = act_eval<A(), false, sizeof(T) == 2>(v[e] + b[e], p.beta, p.inv_beta, slope) + r[e];
                         } else {
-                            act_eval<true>(v[e] + b[e], p.act, p.beta, slope);
+                            act_eval<A(), true, sizeof(T) == 2>(v[e] + b[e], p.beta, p.inv_beta, slope);
                             v[e] = r[e] * slope;
                         }
                     }
                 }
-                store8<T>(p.out + j * p.ld_out + i, v, p.i.n_out - i);
+                store8<T>(p.out + j * p.ld_out + i, v, j < p.j.n_out ? p.i.n_out - i : 0);
             }
         }
+        });
     }
-}
-
-// dw (and the column sums db) = the sums of the slabs' partials, in their order
-template <typename T>
-__global__ void __launch_bounds__(256)
-dense_dw_sum_kernel(const float *__restrict__ partial, int slabs, int64_t n, int64_t n_db, T *__restrict__ dw, T *__restrict__ db) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = n + n_db;
-    if (e >= stride) return;
-    float s[4] = {};
-    int k = 0;
-    for (; k + 3 < slabs; k += 4)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) s[u] += partial[(k + u) * stride + e];
-    for (; k < slabs; ++k) s[0] += partial[k * stride + e];
-    const float v = (s[0] + s[1]) + (s[2] + s[3]);
-    if (e < n) dw[e] = (T)v;
-    else db[e - n] = (T)v;
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------------------
@@ -589,7 +676,8 @@ dense_few_kernel(const DenseArgs<T> p) {
             const T *b = q ? p.bias2 : p.bias;
             if (b) v[q] += (float)b[i];
         }
-        float slope, y = act_eval<false>(v[0], p.act, p.beta, slope);
+        float slope, y = 0.f;
+        with_act(p.act, [&](auto A) { y = act_eval<A(), false, sizeof(T) == 2>(v[0], p.beta, p.inv_beta, slope); });
         if (GATED) y *= v[NG - 1];
         else if (p.res) y += (float)p.res[j * p.ld_res + i];
         p.out[j * p.ld_out + i] = (T)y;
@@ -599,30 +687,53 @@ dense_few_kernel(const DenseArgs<T> p) {
 // ---- launches -------------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kFewRows = 32;
 
-// Tiles: 128 x 128 (four waves of 64 x 64) where they fill the chip, else 64 x 64 (four waves of 64 x 16): a product of few tiles is
-// bound by how many CUs take part.
-template <typename T, int MODE>
-static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
-    constexpr bool GATED = MODE == kGatedFwd || MODE == kGatedBwd;
-    const int64_t oi = GATED ? p.i.n_out * 2 : p.i.n_out;
-    const bool big = ceil_div<int64_t>(oi, 128) * ceil_div<int64_t>(p.j.n_out, 128) * (MODE == kDenseDw ? p.slabs : 1) >= 256;
-    const int b = big ? 128 : 64;
-    p.tiles_i = ceil_div<int64_t>(oi, b);
-    p.tiles = p.tiles_i * ceil_div<int64_t>(p.j.n_out, b) * (MODE == kDenseDw ? p.slabs : 1);
-    const int64_t grid = ceil_div<int64_t>(p.tiles, 8) * 8;
-    if (grid > 0x7fffffff) return einval("dense: too many tiles for one launch");
-    if (big) hipLaunchKernelGGL((dense_kernel<T, MODE, 2, 2, 4, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((dense_kernel<T, MODE, 1, 4, 4, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
-    return check_launch("dense");
-}
-
-// slabs of a weight gradient (rows cut so that the tiles times the slabs fill the chip twice over, none shorter than 256 rows)
-static inline int dense_dw_slabs(int64_t rows, int64_t n, int64_t k) {
-    const int64_t tiles = ceil_div<int64_t>(n, 128) * ceil_div<int64_t>(k, 128);
-    int64_t s = ceil_div<int64_t>(512, tiles);
+// slabs of a weight gradient: the rows are cut so that tiles times slabs fill the chip (256 x 256 tiles: once; 128 x 128: two workgroups to a
+// CU), none shorter than 256 rows.  A rule on sizes and type only: the scratch a caller brings is as large whatever its pointers' alignment.
+// (256 x 256 tiles make twice the partial sums, 64 MB of them, and 1.2 x the rate: 271 against 326 us for a 2048 x 512 weight and 65536 rows;
+// 101 against 96 us for one of 256 x 256 and 262144 rows.)
+static inline bool dense_dw_wide(int elem_bytes, int64_t n, int64_t k) { return elem_bytes == 2 && n >= 256 && k >= 256 && n * k >= 512 * 512; }
+static inline int dense_dw_slabs(int elem_bytes, int64_t rows, int64_t n, int64_t k) {
+    const int64_t b = dense_dw_wide(elem_bytes, n, k) ? 256 : 128;
+    const int64_t tiles = ceil_div<int64_t>(n, b) * ceil_div<int64_t>(k, b);
+    int64_t s = (b == 256 ? 256 : 512) / tiles;
     const int64_t most = ceil_div<int64_t>(rows, 256);
     s = s < most ? s : most;
     return (int)(s > 0 ? s : 1);
+}
+
+// The tile of a product, by how many there would be: the chip takes part with as many CUs as there are tiles, and a larger tile reads less
+// LDS per operation and computes longer on what it has loaded.  (64 x 64: four waves of 64 x 16; 128 x 128: four of 64 x 64, two workgroups
+// to a CU; 256 x 256: eight of 128 x 64, one workgroup - gated backward, with its third accumulator, 256 x 192.)  65536 rows, 512 x 2048, bf16,
+// 256 against 128: gated forward 361 / 472 us, gated backward 728 / 843, input gradient 351 / 398, 2048 -> 512 152 / 180.
+template <typename T, int MODE>
+static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
+    constexpr bool GATED = MODE == kGatedFwd || MODE == kGatedBwd;
+    constexpr bool TR_I = MODE == kDenseDx || MODE == kDenseDw, TR_J = MODE == kDenseDw;
+    const int64_t oi = GATED ? p.i.n_out * 2 : p.i.n_out, z = MODE == kDenseDw ? p.slabs : 1;
+    auto count = [&](int bi, int bj) { return ceil_div<int64_t>(oi, bi) * ceil_div<int64_t>(p.j.n_out, bj) * z; };
+    auto aligned = [](const Operand<T> &q, bool tr) {
+        return ((reinterpret_cast<uintptr_t>(q.a) | reinterpret_cast<uintptr_t>(q.b)) & 15) == 0 && q.ld % 8 == 0 && (!tr || q.n_out % 8 == 0);
+    };
+    const bool async = sizeof(T) == 2 && aligned(p.i, TR_I) && aligned(p.j, TR_J) && (MODE != kGatedBwd || (aligned(p.i2, true) && aligned(p.j2, false)));
+    const bool wide = async && (MODE == kDenseDw ? dense_dw_wide(2, p.j.n_out, p.i.n_out) && count(256, 256) >= 128 : oi >= 256 && count(256, 256) >= 256);
+    const bool big = count(128, 128) >= 256;
+    const int bi = wide ? 256 : big ? 128 : 64, bj = wide ? (MODE == kGatedBwd ? 192 : 256) : bi;
+    p.tiles_i = ceil_div<int64_t>(oi, bi);
+    p.tiles = count(bi, bj);
+    const int64_t grid = ceil_div<int64_t>(p.tiles, 8) * 8;
+    if (grid > 0x7fffffff) return einval("dense: too many tiles for one launch");
+#define ARCN_DK(WI_, WJ_, MI_, NJ_, A_) hipLaunchKernelGGL((dense_kernel<T, MODE, WI_, WJ_, MI_, NJ_, A_>), dim3((unsigned)grid), dim3(64 * WI_ * WJ_), 0, st, p)
+    if constexpr (sizeof(T) == 2) {
+        if (wide) ARCN_DK(2, 4, 8, (MODE == kGatedBwd ? 3 : 4), true);
+        else if (big && async) ARCN_DK(2, 2, 4, 4, true);
+        else if (async) ARCN_DK(1, 4, 4, 1, true);
+    }
+    if (!async) {
+        if (big) ARCN_DK(2, 2, 4, 4, false);
+        else ARCN_DK(1, 4, 4, 1, false);
+    }
+#undef ARCN_DK
+    return check_launch("dense");
 }
 
 template <typename T>

@@ -23,6 +23,7 @@ int DenseOps<T>::fwd(const void *x, int64_t ld_x, const void *w, const void *b, 
     p.ld_out = N;
     p.act = act;
     p.beta = beta;
+    p.inv_beta = 1.f / beta;
     if (rows <= kFewRows) {
         const dim3 grid((unsigned)ceil_div<int>(N, 16));
         if (rows <= 16) hipLaunchKernelGGL((dense_few_kernel<T, false, 1>), grid, dim3(256), 0, st, p);
@@ -45,6 +46,7 @@ int DenseOps<T>::dz(const void *x, int64_t ld_x, const void *w, const void *b, c
     p.ld_out = N;
     p.act = act;
     p.beta = beta;
+    p.inv_beta = 1.f / beta;
     return launch_tiles<T, kDenseDz>(p, st);
 }
 
@@ -65,11 +67,10 @@ int DenseOps<T>::dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, 
     p.j = {tp<T>(dz), nullptr, ld_dz, N, rows, 0};
     p.partial = scratch;
     p.want_sums = db != nullptr;
-    p.slabs = dense_dw_slabs(rows, N, K);
+    p.slabs = dense_dw_slabs(sizeof(T), rows, N, K);
     if (int rc = launch_tiles<T, kDenseDw>(p, st)) return rc;
     const int64_t n = (int64_t)N * K, n_db = db ? N : 0;
-    hipLaunchKernelGGL((dense_dw_sum_kernel<T>), dim3((unsigned)ceil_div<int64_t>(n + n_db, 256)), dim3(256), 0, st, scratch, p.slabs, n, n_db, static_cast<T *>(dw),
-                       static_cast<T *>(db));
+    sum_partials<T>(scratch, p.slabs, n, n_db, static_cast<T *>(dw), static_cast<T *>(db), st);
     return check_launch("dense_dw");
 }
 
@@ -85,6 +86,7 @@ int DenseOps<T>::gated_fwd(const void *x, int64_t ld_x, const void *wg, const vo
     p.ld_out = H;
     p.act = act;
     p.beta = beta;
+    p.inv_beta = 1.f / beta;
     if (rows <= kFewRows) {
         const dim3 grid((unsigned)ceil_div<int>(H, 16));
         if (rows <= 16) hipLaunchKernelGGL((dense_few_kernel<T, true, 1>), grid, dim3(256), 0, st, p);
@@ -108,6 +110,7 @@ int DenseOps<T>::gated_bwd(const void *x, int64_t ld_x, const void *wg, const vo
     p.ld_out = 2 * (int64_t)H;
     p.act = act;
     p.beta = beta;
+    p.inv_beta = 1.f / beta;
     return launch_tiles<T, kGatedBwd>(p, st);
 }
 

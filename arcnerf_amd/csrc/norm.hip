@@ -12,6 +12,7 @@
 //
 // Bound by HBM: 2 (forward) and 3 (backward) row-sized streams.
 #include "elem.hpp"
+#include "partials.hpp"
 
 #pragma clang fp contract(fast)
 
@@ -227,44 +228,15 @@ layer_norm_dw_wide_kernel(const T *__restrict__ x, int64_t ld_x, const T *__rest
     partial[(int64_t)blockIdx.x * 2 * C + C + c] = db;
 }
 
-// dweight / dbias = the sums of the n_part partial rows, in a fixed order: 32 columns x 8 interleaved shares of the rows per workgroup
-template <typename WT>
-__global__ void __launch_bounds__(kNormThreads)
-layer_norm_dw_sum_kernel(const float *__restrict__ partial, int n_part, int C, WT *__restrict__ dw, WT *__restrict__ db) {
-    __shared__ float lds[8][33];
-    const int lc = threadIdx.x & 31, share = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + lc;
-    float s[4] = {};
-    if (col < 2 * (int64_t)C) {
-        int p = share;
-        for (; p + 24 < n_part; p += 32)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] += partial[(int64_t)(p + 8 * u) * 2 * C + col];
-        for (; p < n_part; p += 8) s[0] += partial[(int64_t)p * 2 * C + col];
-    }
-    lds[share][lc] = (s[0] + s[1]) + (s[2] + s[3]);
-    __syncthreads();
-    if (share == 0 && col < 2 * (int64_t)C) {
-        float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v += lds[k][lc];
-        if (col < C) {
-            if (dw) dw[col] = (WT)v;
-        } else if (db) {
-            db[col - C] = (WT)v;
-        }
-    }
-}
-
 // workgroups of a register kernel: rows_per = rows per workgroup and trip
 static inline unsigned norm_grid(int64_t rows, int rows_per, int most) {
     const int64_t g = ceil_div<int64_t>(rows, rows_per);
     return (unsigned)(g < most ? g : most);
 }
 
-static inline int norm_lpr(int dtype, int C) {
+static inline int norm_lpr(int dtype, int C) {      // as norm_shape has it
     const int nv = ceil_div<int>(C, dtype == ARCN_DTYPE_F32 ? 4 : 8);
-    return nv <= 8 ? 8 : nv <= 16 ? 16 : nv <= 32 ? 32 : C <= 2048 ? 64 : 256;
+    return nv <= 8 ? 8 : nv <= 16 ? 16 : nv <= (dtype == ARCN_DTYPE_F32 ? 32 : 64) ? 32 : C <= 2048 ? 64 : 256;
 }
 
 static inline int norm_parts(int64_t rows, int dtype, int C) {
@@ -290,7 +262,7 @@ static void norm_shape(int C, Fn &&f) {
         if (C <= 64) ARCN_NS(8, 1);
         else if (C <= 128) ARCN_NS(16, 1);
         else if (C <= 256) ARCN_NS(32, 1);
-        else if (C <= 512) ARCN_NS(64, 1);
+        else if (C <= 512) ARCN_NS(32, 2);      // two rows to a wave
         else if (C <= 1024) ARCN_NS(64, 2);
         else if (C <= 2048) ARCN_NS(64, 4);
         else if (C <= 4096) ARCN_NS(256, 2);
@@ -337,8 +309,7 @@ static void norm_bwd(const void *x, int64_t ld_x, const void *dy, int64_t ld_dy,
         });
     }
     if (part)
-        hipLaunchKernelGGL((layer_norm_dw_sum_kernel<WT>), dim3((unsigned)ceil_div<int64_t>(2 * (int64_t)C, 32)), dim3(kNormThreads), 0, st, part, parts, C,
-                           static_cast<WT *>(dw), static_cast<WT *>(db));
+        sum_partials<WT>(part, parts, C, C, static_cast<WT *>(dw), static_cast<WT *>(db), st);
 }
 
 static int norm_args(const char *what, int dtype, int w_dtype, int64_t n_rows, int C) {

@@ -1332,7 +1332,7 @@ def dense_dw(dz, x, want_db=False):
     (S, K), Nn = x.shape, dz.shape[1]
     dw = _fresh((Nn, K), x.dtype, x.device)
     db = _fresh((Nn,), x.dtype, x.device) if want_db else None
-    nf = int(N.lib().arcn_dense_dw_scratch_floats(S, Nn, K))
+    nf = int(N.lib().arcn_dense_dw_scratch_floats(S, Nn, K, _DTYPE[x.dtype]))
     scratch = torch.empty(nf, dtype=torch.float32, device=x.device)
     with _device_of(x):
         N.check(N.lib().arcn_dense_dw(dz.data_ptr(), ld, x.data_ptr(), ld_x, N.ptr(dw), N.ptr(db), _DTYPE[x.dtype], N.ptr(scratch), nf, S, Nn, K, N.stream()),

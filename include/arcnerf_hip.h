@@ -839,7 +839,7 @@ int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, 
 /* dx (n_rows, K) = dz (n_rows, N) w (N, K).  w2 not NULL (N even): the weight's first N / 2 rows are w (N / 2, K), the others w2. */
 int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int dtype, int64_t n_rows, int N, int K, void *stream);
 /* dw (N, K) = dz^T x and, unless db is NULL, db (N) = the column sums of dz.  scratch: arcn_dense_dw_scratch_floats floats. */
-int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K);
+int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K, int dtype);
 int arcn_dense_dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, int dtype, float *scratch, int64_t scratch_floats,
                   int64_t n_rows, int N, int K, void *stream);
 /* h (n_rows, H) = act(x w_gate^T + b_gate) * (x w_up^T + b_up); w_gate and w_up (H, K), biases (H) or NULL */
