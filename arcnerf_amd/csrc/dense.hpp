@@ -123,7 +123,7 @@ struct Mma;
 template <>
 struct Mma<__bf16> {
     static constexpr int P = 1, BK = 64, NBUF = 2;
-    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c) {
+    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c, float) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[0]), __builtin_bit_cast(bf16x8, b[0]), c, 0, 0, 0);
     }
     static constexpr short kOne = 0x3f80;
@@ -131,7 +131,7 @@ struct Mma<__bf16> {
 template <>
 struct Mma<_Float16> {
     static constexpr int P = 1, BK = 64, NBUF = 2;
-    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c) {
+    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c, float) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c, 0, 0, 0);
     }
     static constexpr short kOne = 0x3c00;
@@ -142,16 +142,20 @@ struct Mma<float> {
     static __device__ __forceinline__ f4v one(s8v a, s8v b, f4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    // the six terms of 32 reduction elements among themselves, smallest first, then ONE addition (rounded to nearest) to the running sum:
-    // six accumulations straight into it would round at its size six times
-    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c) {
+    // The six terms of 32 reduction elements among themselves, smallest first, then ONE addition (rounded to nearest) to the running sum:
+    // six accumulations straight into it would round at its size six times.  The matrix cores round their sums downwards, a bias that
+    // adds up in a column sum over many rows: the I operand of every other step comes negated (sign = -1), which turns it around.
+    static __device__ __forceinline__ f4v mma(const s8v *a, const s8v *b, f4v c, float sign) {
         f4v t = {0.f, 0.f, 0.f, 0.f};
         t = one(a[1], b[1], t);
         t = one(a[0], b[2], t);
         t = one(a[2], b[0], t);
         t = one(a[0], b[1], t);
         t = one(a[1], b[0], t);
-        return c + one(a[0], b[0], t);
+        t = one(a[0], b[0], t);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] = fmaf(sign, t[r], c[r]);
+        return c;
     }
     static constexpr short kOne = 0x3f80;
 };
@@ -189,12 +193,14 @@ __device__ __forceinline__ void store8(T *p, const float *v, int64_t left) {
 
 // the planes of eight elements: themselves for the 16-bit types; hi, mid, lo for f32 (each rounded to nearest: the remainders are exact)
 template <typename T>
-__device__ __forceinline__ void planes8(const Raw8<T> &r, s8v *pl) {
+__device__ __forceinline__ void planes8(const Raw8<T> &r, s8v *pl, float sign = 1.f) {
     if constexpr (sizeof(T) == 2) {
         pl[0] = __builtin_bit_cast(s8v, r.v[0]);
     } else {
         float v[8];
         unpack8<T>(r, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= sign;
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
             const u4v q = Elem<__bf16>::pack(v);
@@ -258,13 +264,13 @@ struct Tile {
         }
     }
 
-    __device__ __forceinline__ void stash(short *lds, int tid) {
+    __device__ __forceinline__ void stash(short *lds, int tid, float sign = 1.f) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int q = tid + n * THREADS;
             if (CHUNKS % THREADS && q >= CHUNKS) break;
             s8v pl[P];
-            planes8<T>(raw[n], pl);
+            planes8<T>(raw[n], pl, sign);
 #pragma unroll
             for (int p = 0; p < P; ++p) *reinterpret_cast<s8v *>(lds + p * R * BK + place(q / PER_ROW, q % PER_ROW)) = pl[p];
         }
@@ -398,7 +404,7 @@ dense_kernel(const DenseArgs<T> p) {
     };
     if (RES_EARLY && p.res) fetch_res();
 
-    auto step = [&](auto &ti, auto &tj, const short *buf, auto &c) {
+    auto step = [&](auto &ti, auto &tj, const short *buf, auto &c, float sign = 1.f) {
         typedef std::remove_reference_t<decltype(ti)> Ti;
         typedef std::remove_reference_t<decltype(tj)> Tj;
         constexpr int M = sizeof(c) / sizeof(c[0]);
@@ -412,14 +418,14 @@ dense_kernel(const DenseArgs<T> p) {
                 s8v a[P];
                 Ti::frag(buf, wi * 16 * M, m, kk, lane, a);
 #pragma unroll
-                for (int n = 0; n < NJ; ++n) c[m][n] = Mma<T>::mma(a, b[n], c[m][n]);
+                for (int n = 0; n < NJ; ++n) c[m][n] = Mma<T>::mma(a, b[n], c[m][n], sign);
             }
             if (MODE == kDenseDw && my_sums) {
                 const short one = Mma<T>::kOne;
                 s8v ones[P] = {};
                 ones[0] = s8v{one, one, one, one, one, one, one, one};
 #pragma unroll
-                for (int n = 0; n < NJ; ++n) sums[n] = Mma<T>::mma(ones, b[n], sums[n]);
+                for (int n = 0; n < NJ; ++n) sums[n] = Mma<T>::mma(ones, b[n], sums[n], 1.f);
             }
         }
     };
@@ -432,14 +438,15 @@ dense_kernel(const DenseArgs<T> p) {
             }
             for (int64_t s = 0; s < n_steps; ++s) {
                 const int64_t k = k_lo + (s + 1) * BK;
-                ti.stash(lds, tid);
+                const float sign = s & 1 ? -1.f : 1.f;
+                ti.stash(lds, tid, sign);
                 tj.stash(lds + TI::kElems, tid);
                 __syncthreads();
                 if (s + 1 < n_steps) {
                     ti.fetch(oi, i0, k, k_hi, tid);
                     tj.fetch(oj, j0, k, k_hi, tid);
                 }
-                step(ti, tj, lds, c);
+                step(ti, tj, lds, c, sign);
                 __syncthreads();
             }
         } else {
@@ -645,7 +652,7 @@ dense_few_kernel(const DenseArgs<T> p) {
 #pragma unroll
         for (int q = 0; q < NG; ++q)
 #pragma unroll
-            for (int n = 0; n < NJ; ++n) acc[q][n] = Mma<T>::mma(a[q], b[n], acc[q][n]);
+            for (int n = 0; n < NJ; ++n) acc[q][n] = Mma<T>::mma(a[q], b[n], acc[q][n], 1.f);
     };
     const int64_t n_full = K / 32;   // whole steps of 32
     int64_t s = wave;

@@ -11,6 +11,7 @@ import torch.nn as nn
 from ....utils.cfgs_utils import dict_to_obj
 from ....utils.registry import MODULE_REGISTRY
 from ..activation import get_activation
+from ..ffn import build_block
 from ..linear import DenseLayer, Linear, SirenLayer
 from .encoder_mlp_network import EncoderMLPGeoNet, EncoderMLPRadainceNet
 
@@ -21,7 +22,7 @@ from .encoder_mlp_network import EncoderMLPGeoNet, EncoderMLPRadainceNet
 class GeoNet(EncoderMLPGeoNet):
     def __init__(self, W=256, D=8, skips=[4], encoder=None, W_feat=256, use_bias=True, skip_reduce_output=False,
                  norm_skip=False, act_cfg=None, geometric_init=True, radius_init=1.0, use_siren=False, weight_norm=False,
-                 out_act_cfg=None, *args, **kwargs):
+                 out_act_cfg=None, block_cfg=None, *args, **kwargs):
         super().__init__(W_feat=W_feat, out_act_cfg=out_act_cfg)
         self.W, self.D, self.skips, self.norm_skip = W, D, list(skips), norm_skip
         self.geometric_init, self.use_siren, self.radius_init = geometric_init, use_siren, radius_init
@@ -29,6 +30,9 @@ class GeoNet(EncoderMLPGeoNet):
         input_ch, embed_freq = self.build_encoder(encoder)
         if use_siren:
             assert len(self.skips) == 0, 'do not use skips for siren'
+        if block_cfg is not None:
+            # hidden layers 1 .. D - 1 as residual blocks (base_modules/ffn.py): the residual takes the place of the skip concatenation
+            assert len(self.skips) == 0 and not use_siren and not weight_norm, 'residual blocks take no skips, siren or weight norm'
         layers = []
         for i in range(D + 1):
             after_skip = i > 0 and (i - 1) in self.skips
@@ -39,6 +43,9 @@ class GeoNet(EncoderMLPGeoNet):
                 out_dim = W - self.embed_dim
             else:
                 out_dim = W
+            if block_cfg is not None and 0 < i < D:
+                layers.append(build_block(block_cfg, W, bias=use_bias))
+                continue
             if i == D:
                 layer = Linear(in_dim, out_dim, bias=use_bias)
             elif use_siren:
@@ -145,12 +152,17 @@ class GeoNet(EncoderMLPGeoNet):
 @MODULE_REGISTRY.register()
 class RadianceNet(EncoderMLPRadainceNet):
     def __init__(self, mode='vf', W=256, D=8, encoder=None, W_feat_in=256, use_bias=True, act_cfg=None, use_siren=False,
-                 weight_norm=False, out_act_cfg=None, *args, **kwargs):
+                 weight_norm=False, out_act_cfg=None, block_cfg=None, *args, **kwargs):
         super().__init__(mode=mode)
         self.W, self.D, self.W_feat_in = W, D, W_feat_in
         self.build_encoder(encoder, W_feat_in)
+        if block_cfg is not None:
+            assert not use_siren and not weight_norm, 'residual blocks take no siren or weight norm'
         layers = []
         for i in range(D + 1):
+            if block_cfg is not None and 0 < i < D:
+                layers.append(build_block(block_cfg, W, bias=use_bias))
+                continue
             in_dim = self.init_input_dim if i == 0 else W
             if i == D:
                 act = get_activation(out_act_cfg, dict_to_obj({'type': 'Sigmoid'}))
