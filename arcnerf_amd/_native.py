@@ -11,6 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(_HERE)
 HEADER = os.path.join(ROOT, 'include', 'arcnerf_hip.h')
 LIB_PATH = os.path.join(_HERE, 'lib', 'libarcnerf_hip.so')
+NODES_PATH = os.path.join(_HERE, 'lib', 'arcnerf_torch.so')
 
 MAX_LEVELS = 32
 ACT = {None: 0, 'none': 0, 'relu': 1, 'sigmoid': 2, 'truncexp': 3, 'exponential': 3, 'softplus': 4, 'squareplus': 5, 'sine': 6}
@@ -70,6 +71,28 @@ def lib():
             fn.argtypes = argtypes
         _lib = handle
     return _lib
+
+
+_nodes = None
+
+
+def torch_nodes():
+    """The extension module with the feed-forward layers' autograd nodes (csrc/torch_nodes.cpp; once).  Raises RuntimeError if it has not been
+    built: there is no Python form of them."""
+    global _nodes
+    if _nodes is None:
+        if not os.path.exists(NODES_PATH):
+            raise RuntimeError('arcnerf_torch.so is not built ({}); run `python -c "import __graft_entry__ as g; g.build()"` or '
+                               '`make -C arcnerf_amd/csrc`'.format(NODES_PATH))
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries are the extension's)
+        lib()
+        spec = importlib.util.spec_from_file_location('arcnerf_torch', NODES_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _nodes = module
+    return _nodes
 
 
 def check(rc, what=''):

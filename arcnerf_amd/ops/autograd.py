@@ -6,6 +6,7 @@ every Function is one forward kernel and one backward kernel.
 import torch
 from torch.autograd.function import once_differentiable
 
+from .. import _native as N
 from . import functional as F
 
 
@@ -843,38 +844,11 @@ def linear(x, weight, bias=None, keep_pad=False):
 
 
 # ------------------------------------------------------------------------------------------------------------------------------------
-# Residual feed-forward layers, float32 / bfloat16 / float16 (csrc/norm.hip, csrc/dense.hpp).  First order: a second differentiation raises.
-# CPU tensors (host-side tests of the modules) go to torch, as in `linear`.
+# Residual feed-forward layers, float32 / bfloat16 / float16 (csrc/norm.hip, csrc/dense.hpp; the nodes are csrc/torch_nodes.cpp, which also
+# checks shapes, types and devices and raises RuntimeError).  First order: differentiating a gradient again raises.  A backward pass keeps the
+# inputs only (layer norm: and its rows' statistics; the gated block: and the product of its gate).  CPU tensors (host-side tests of the
+# modules) go to torch, as in `linear`.
 # ------------------------------------------------------------------------------------------------------------------------------------
-def _needs_graph(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _rows_of(name, x, width):
-    if x.dim() < 1 or x.shape[-1] != width:
-        raise RuntimeError('arcnerf_amd: {} must be (..., {}), got {}'.format(name, width, tuple(x.shape)))
-    return x if x.dim() == 2 else x.reshape(-1, width)
-
-
-class LayerNormFn(torch.autograd.Function):
-    """layer norm of the rows of x (S, C); keeps x and the rows' statistics"""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = F.layer_norm_fwd(x, weight, bias, eps, want_stats=True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.param_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, stats = ctx.saved_tensors
-        want_dx, want_dw, want_db = ctx.needs_input_grad[:3]
-        dx, dw, db = F.layer_norm_bwd(x, g, weight, stats, want_dx, want_dw, want_db, ctx.param_dtype)
-        return dx, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of x: (x - mean) / sqrt(var + eps) * weight + bias.  x float32, bfloat16 or float16; weight and
     bias (C) of x's type or both float32, either may be None.  Statistics and sums in float32."""
@@ -882,109 +856,32 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         C = x.shape[-1]
         y = torch.nn.functional.layer_norm(x.float(), (C,), None if weight is None else weight.float(), None if bias is None else bias.float(), eps)
         return y.to(x.dtype)
-    x2 = _rows_of('x', x, x.shape[-1] if x.dim() else 0)
-    y = LayerNormFn.apply(x2, weight, bias, float(eps)) if _needs_graph(x, weight, bias) else F.layer_norm_fwd(x2, weight, bias, eps)
-    return y.view(x.shape)
+    return N.torch_nodes().layer_norm(x, weight, bias, eps)
 
 
-def _host_act(z, act, beta):
+def _host_act(z, code, beta):
     fn = torch.nn.functional
     return {0: lambda: z, 1: lambda: fn.relu(z), 2: lambda: torch.sigmoid(z), 4: lambda: fn.softplus(z, beta=beta), 7: lambda: fn.silu(z),
-            8: lambda: fn.gelu(z)}[F._dense_act(act, beta)]()
-
-
-class LinearActResidualFn(torch.autograd.Function):
-    """y = act(x @ w.T + bias) + residual on rows; keeps the inputs only, the backward computes the pre-activation again"""
-
-    @staticmethod
-    def forward(ctx, x, w, bias, residual, act, beta):
-        ctx.save_for_backward(x, w, bias)
-        ctx.act, ctx.beta = act, beta
-        return F.dense_fwd(x, w, bias, residual, act, beta)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, w, bias = ctx.saved_tensors
-        want_dx, want_dw, want_db, want_dr = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if want_dx or want_dw or want_db:
-            dz = F.dense_dz(x, w, bias, g, ctx.act, ctx.beta)
-            dx = F.dense_dx(dz, w) if want_dx else None
-            if want_dw or want_db:
-                dw, db = F.dense_dw(dz, x, want_db=want_db)
-        return dx, (dw if want_dw else None), db, (g if want_dr else None), None, None
+            8: lambda: fn.gelu(z)}[code]()
 
 
 def linear_act_residual(x, weight, bias=None, residual=None, act=None, beta=1.0):
     """act(x @ weight.T + bias) + residual as one product with an epilogue: x (..., K), weight (N, K), bias (N), residual (..., N) like the
-    result; one type for all of them, float32, bfloat16 or float16.  act: None, relu, sigmoid, softplus (beta), silu, gelu."""
-    n_out, k_in = weight.shape
+    result; one type for all of them, float32, bfloat16 or float16.  act: None, relu, sigmoid, softplus (beta), silu, gelu.  Infinities and NaN in
+    float32 operands give NaN."""
+    code = F._dense_act(act, beta)
     if not x.is_cuda:
-        y = _host_act(torch.nn.functional.linear(x, weight, bias), act, beta)
+        y = _host_act(torch.nn.functional.linear(x, weight, bias), code, beta)
         return y if residual is None else y + residual
-    shape = x.shape[:-1] + (n_out,)
-    if residual is not None and residual.shape != shape:
-        raise RuntimeError('arcnerf_amd: the residual must be {}, got {}'.format(tuple(shape), tuple(residual.shape)))
-    x2 = _rows_of('x', x, k_in)
-    r2 = None if residual is None else _rows_of('residual', residual, n_out)
-    if _needs_graph(x, weight, bias, residual):
-        y = LinearActResidualFn.apply(x2, weight, bias, r2, act, float(beta))
-    else:
-        y = F.dense_fwd(x2, weight, bias, r2, act, beta)
-    return y.view(shape)
-
-
-class GatedFfnFn(torch.autograd.Function):
-    """y = (act(x @ wg.T + bg) * (x @ wu.T + bu)) @ wd.T + bd + residual on rows; keeps the inputs and the product h of the gate, the
-    backward computes both pre-activations again in the kernel that needs them"""
-
-    @staticmethod
-    def forward(ctx, x, wg, wu, wd, bg, bu, bd, residual, act, beta):
-        h = F.gated_fwd(x, wg, wu, bg, bu, act, beta)
-        ctx.save_for_backward(x, wg, wu, wd, bg, bu, h)
-        ctx.act, ctx.beta = act, beta
-        return F.dense_fwd(h, wd, bd, residual)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, wg, wu, wd, bg, bu, h = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dwg = dwu = dwd = dbg = dbu = dbd = None
-        if need[3] or need[6]:
-            dwd, dbd = F.dense_dw(g, h, want_db=need[6])
-        inner_w, inner_b = need[1] or need[2], need[4] or need[5]
-        if need[0] or inner_w or inner_b:
-            dgu = F.gated_bwd(x, wg, wu, bg, bu, g, wd, ctx.act, ctx.beta)
-            if need[0]:
-                dx = F.dense_dx(dgu, wg, wu)
-            if inner_w or inner_b:
-                H = wg.shape[0]
-                dw, db = F.dense_dw(dgu, x, want_db=inner_b)
-                dwg, dwu = dw[:H], dw[H:]
-                if inner_b:
-                    dbg, dbu = db[:H], db[H:]
-        grads = (dx, dwg, dwu, dwd, dbg, dbu, dbd, g)
-        return tuple(v if want else None for v, want in zip(grads, need)) + (None, None)
+    return N.torch_nodes().linear_act_residual(x, weight, bias, residual, code, beta)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, residual=None, act='silu', beta=1.0):
     """The gated feed-forward block (act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)) @ w_down.T + b_down + residual: x (..., K), w_gate and
-    w_up (H, K), w_down (N, H), residual (..., N); one type for all of them.  The product of the gate is held in that type."""
-    hid, k_in = w_gate.shape
-    n_out = w_down.shape[0]
+    w_up (H, K), w_down (N, H), residual (..., N); one type for all of them, in which the product of the gate is held too."""
+    code = F._dense_act(act, beta)
     if not x.is_cuda:
         lin = torch.nn.functional.linear
-        y = lin(_host_act(lin(x, w_gate, b_gate), act, beta) * lin(x, w_up, b_up), w_down, b_down)
+        y = lin(_host_act(lin(x, w_gate, b_gate), code, beta) * lin(x, w_up, b_up), w_down, b_down)
         return y if residual is None else y + residual
-    shape = x.shape[:-1] + (n_out,)
-    if residual is not None and residual.shape != shape:
-        raise RuntimeError('arcnerf_amd: the residual must be {}, got {}'.format(tuple(shape), tuple(residual.shape)))
-    x2 = _rows_of('x', x, k_in)
-    r2 = None if residual is None else _rows_of('residual', residual, n_out)
-    if _needs_graph(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual):
-        y = GatedFfnFn.apply(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, r2, act, float(beta))
-    else:
-        y = F.dense_fwd(F.gated_fwd(x2, w_gate, w_up, b_gate, b_up, act, beta), w_down, b_down, r2)
-    return y.view(shape)
+    return N.torch_nodes().gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, code, beta)
