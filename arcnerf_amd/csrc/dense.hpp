@@ -180,6 +180,19 @@ __device__ __forceinline__ Raw8<T> load8(const T *p, int64_t left) {   // `left`
     for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = load_pack(p + h * Elem<T>::VEC, left - h * Elem<T>::VEC);
     return r;
 }
+// the branch-free form (rows of at least 8 elements): tail8 loads, tail8_fix puts in place
+template <typename T>
+__device__ __forceinline__ Raw8<T> tail8(const T *p, int64_t left) {
+    Raw8<T> r;
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = load16(tail_at<T>(p + h * Elem<T>::VEC, left - h * Elem<T>::VEC));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void tail8_fix(Raw8<T> &r, int64_t left) {
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(T) / 2; ++h) r.v[h] = tail_fix<T>(r.v[h], left - h * Elem<T>::VEC);
+}
 template <typename T>
 __device__ __forceinline__ void unpack8(const Raw8<T> &r, float *v) {
 #pragma unroll
@@ -251,24 +264,57 @@ struct Tile {
         return (op.b && r >= op.split ? op.b + (r - op.split) * op.ld : op.a + r * op.ld) + out0 + 8 * c;
     }
 
+    // How a step is loaded (the same for the whole workgroup): all of it there; some of it behind an end of the operand, rows of 8 elements or
+    // more (no branches: a lane that waited for its tail would hold up the loads of the wave); narrow rows, element by element.
+    enum How { kWhole, kTail, kNarrow };
+    static __device__ __forceinline__ How how(const Operand<T> &op, int64_t out0, int64_t k0, int64_t k_end) {
+        if (k0 + BK <= k_end && (!TR || out0 + R <= op.n_out)) return kWhole;
+        return (TR ? op.n_out : op.n_red) >= 8 ? kTail : kNarrow;
+    }
+    // elements of its row from chunk c of LDS row `row` on; 0 or less: none
+    static __device__ __forceinline__ int64_t left(const Operand<T> &op, int64_t out0, int64_t k0, int64_t k_end, int row, int c) {
+        return TR ? (k0 + row < k_end ? op.n_out - (out0 + 8 * c) : 0) : k_end - (k0 + 8 * c);
+    }
+
     __device__ __forceinline__ void fetch(const Operand<T> &op, int64_t out0, int64_t k0, int64_t k_end, int tid) {
-        const bool full = k0 + BK <= k_end && (!TR || out0 + R <= op.n_out);
+        const How h = how(op, out0, k0, k_end);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int q = tid + n * THREADS;
             if (CHUNKS % THREADS && q >= CHUNKS) break;
             const int row = q / PER_ROW, c = q % PER_ROW;
-            const T *p = source(op, out0, k0, row, c);
-            if (full) raw[n] = load8<T>(p);
-            else raw[n] = load8<T>(p, TR ? (k0 + row < k_end ? op.n_out - (out0 + 8 * c) : 0) : k_end - (k0 + 8 * c));
+            if (h == kWhole) {
+                raw[n] = load8<T>(source(op, out0, k0, row, c));
+            } else if (h == kTail) {
+                // (a reduction row behind the last one reads the last one; stash makes it zero)
+                const int at = TR && k0 + row >= k_end ? (int)(k_end - 1 - k0) : row;
+                raw[n] = tail8<T>(source(op, out0, k0, at, c), left(op, out0, k0, k_end, at, c));
+            } else {
+                raw[n] = load8<T>(source(op, out0, k0, row, c), left(op, out0, k0, k_end, row, c));
+            }
         }
     }
 
-    __device__ __forceinline__ void stash(short *lds, int tid, float sign = 1.f) {
+    // sums (TR, f32; or NULL): the thread's 8 output indices' sums over the rows that it loads (its chunk is the same in all of them)
+    __device__ __forceinline__ void stash(const Operand<T> &op, int64_t out0, int64_t k0, int64_t k_end, short *lds, int tid, float sign = 1.f, float *sums = nullptr) {
+        if (how(op, out0, k0, k_end) == kTail) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int q = tid + n * THREADS;
+                tail8_fix<T>(raw[n], left(op, out0, k0, k_end, q / PER_ROW, q % PER_ROW));
+            }
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int q = tid + n * THREADS;
             if (CHUNKS % THREADS && q >= CHUNKS) break;
+            if (TR && P == 3 && sums) {
+                static_assert(THREADS % PER_ROW == 0, "a thread keeps its chunk");
+                float v[8];
+                unpack8<T>(raw[n], v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sums[e] += v[e];
+            }
             s8v pl[P];
             planes8<T>(raw[n], pl, sign);
 #pragma unroll
@@ -329,16 +375,13 @@ struct DenseArgs {
     int want_sums;
     int act;
     float beta, inv_beta;
-    int64_t tiles_i, tiles;  // tiles: of the whole product (times the slabs)
+    uint32_t tiles_i, tiles_j, tiles;  // tiles: of the whole product (times the slabs)
     int slabs;
 };
 
 // blockIdx -> tile: workgroups are dealt to the 8 XCDs in turn, so each XCD gets a contiguous range of tiles and the tiles that share
 // their J rows (the large operand) meet in one L2
-__device__ __forceinline__ int64_t xcd_tile() {
-    const int64_t per = gridDim.x >> 3;
-    return (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-}
+__device__ __forceinline__ uint32_t xcd_tile() { return (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
 
 // ASYNC: operands straight from memory to LDS (Tile::copy; launch_tiles checks what it needs)
 template <typename T, int MODE, int WI, int WJ, int MI, int NJ, bool ASYNC>
@@ -355,31 +398,35 @@ dense_kernel(const DenseArgs<T> p) {
     constexpr int BUF = TI::kElems + TJ::kElems;
     __shared__ __attribute__((aligned(16))) short lds[NBUF * BUF];
 
-    const int64_t t = xcd_tile();
+    const uint32_t t = xcd_tile();
     if (t >= p.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wi = wave % WI, wj = wave / WI;
-    const int64_t i0 = (t % p.tiles_i) * OUT_I;
-    int64_t rest = t / p.tiles_i, slab = 0, k_lo = 0, k_hi = p.i.n_red;
+    uint32_t rest = t / p.tiles_i;
+    const int64_t i0 = (int64_t)(t - rest * p.tiles_i) * OUT_I;
+    int64_t slab = 0, k_lo = 0, k_hi = p.i.n_red;
     if (MODE == kDenseDw) {
-        const int64_t tiles_j = p.tiles / p.tiles_i / p.slabs;
-        slab = rest / tiles_j;
-        rest %= tiles_j;
+        slab = rest / p.tiles_j;
+        rest -= (uint32_t)slab * p.tiles_j;
         const int64_t per = (ceil_div_dev(p.i.n_red, p.slabs) + BK - 1) / BK * BK;
         k_lo = slab * per;
         k_hi = k_lo + per < p.i.n_red ? k_lo + per : p.i.n_red;
     }
-    const int64_t j0 = rest * BJ;
+    const int64_t j0 = (int64_t)rest * BJ;
 
     f4v acc[MI][NJ];
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int n = 0; n < NJ; ++n) acc[m][n] = f4v{0.f, 0.f, 0.f, 0.f};
-    f4v sums[MODE == kDenseDw ? NJ : 1];
+    // column sums of the J operand (the bias gradient), by the tiles of the first i: 16-bit types by a product with ones (the waves of the first
+    // wi), f32 as its rows are staged (8 registers instead of 16)
+    constexpr bool SUM_MMA = MODE == kDenseDw && P == 1, SUM_ADD = MODE == kDenseDw && P == 3;
+    f4v sums[SUM_MMA ? NJ : 1];
+    float add_sums[SUM_ADD ? 8 : 1] = {};
 #pragma unroll
-    for (int n = 0; n < (MODE == kDenseDw ? NJ : 1); ++n) sums[n] = f4v{0.f, 0.f, 0.f, 0.f};
-    const bool my_sums = MODE == kDenseDw && p.want_sums && i0 == 0 && wi == 0;   // wave-uniform
+    for (int n = 0; n < (SUM_MMA ? NJ : 1); ++n) sums[n] = f4v{0.f, 0.f, 0.f, 0.f};
+    const bool my_sums = MODE == kDenseDw && p.want_sums && i0 == 0 && (wi == 0 || SUM_ADD);   // wave-uniform
 
     // after the swap a lane holds 8 features of a pair of tiles from 32 pr + f8, row o
     const int g = lane >> 4, o = lane & 15, f8 = 16 * (g & 1) + 8 * (g >> 1);
@@ -398,18 +445,20 @@ dense_kernel(const DenseArgs<T> p) {
                     const int64_t i = i0 + wi * 16 * MI + 32 * pr + f8, j = j0 + (wj * NJ + n) * 16 + o;
                     const T *src = p.res + j * p.ld_res + i;
                     if (inner) res[pr][n] = load8<T>(src);
+                    else if (p.i.n_out >= 8) res[pr][n] = tail8<T>(j < p.j.n_out ? src : src + (p.j.n_out - 1 - j) * p.ld_res, p.i.n_out - i);
                     else res[pr][n] = load8<T>(src, j < p.j.n_out ? p.i.n_out - i : 0);
                 }
         }
     };
     if (RES_EARLY && p.res) fetch_res();
 
-    auto step = [&](auto &ti, auto &tj, const short *buf, auto &c, float sign = 1.f) {
+    auto step = [&](auto &ti, auto &tj, const short *buf, auto &c, int64_t k_left, float sign = 1.f) {
         typedef std::remove_reference_t<decltype(ti)> Ti;
         typedef std::remove_reference_t<decltype(tj)> Tj;
         constexpr int M = sizeof(c) / sizeof(c[0]);
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
+            if (kk > 0 && 32 * kk >= k_left) break;
             s8v b[NJ][P];
 #pragma unroll
             for (int n = 0; n < NJ; ++n) Tj::frag(buf + TI::kElems, wj * 16 * NJ, n, kk, lane, b[n]);
@@ -420,7 +469,7 @@ dense_kernel(const DenseArgs<T> p) {
 #pragma unroll
                 for (int n = 0; n < NJ; ++n) c[m][n] = Mma<T>::mma(a, b[n], c[m][n], sign);
             }
-            if (MODE == kDenseDw && my_sums) {
+            if (SUM_MMA && my_sums) {
                 const short one = Mma<T>::kOne;
                 s8v ones[P] = {};
                 ones[0] = s8v{one, one, one, one, one, one, one, one};
@@ -439,14 +488,14 @@ dense_kernel(const DenseArgs<T> p) {
             for (int64_t s = 0; s < n_steps; ++s) {
                 const int64_t k = k_lo + (s + 1) * BK;
                 const float sign = s & 1 ? -1.f : 1.f;
-                ti.stash(lds, tid, sign);
-                tj.stash(lds + TI::kElems, tid);
+                ti.stash(oi, i0, k - BK, k_hi, lds, tid, sign);
+                tj.stash(oj, j0, k - BK, k_hi, lds + TI::kElems, tid, 1.f, SUM_ADD && my_sums ? add_sums : nullptr);
                 __syncthreads();
                 if (s + 1 < n_steps) {
                     ti.fetch(oi, i0, k, k_hi, tid);
                     tj.fetch(oj, j0, k, k_hi, tid);
                 }
-                step(ti, tj, lds, c, sign);
+                step(ti, tj, lds, c, BK, sign);
                 __syncthreads();
             }
         } else {
@@ -457,8 +506,8 @@ dense_kernel(const DenseArgs<T> p) {
                 tj.fetch(oj, j0, k_lo + s * BK, k_hi, tid);
             };
             auto put = [&](int64_t s) {
-                ti.stash(lds + (s & 1) * BUF, tid);
-                tj.stash(lds + (s & 1) * BUF + TI::kElems, tid);
+                ti.stash(oi, i0, k_lo + s * BK, k_hi, lds + (s & 1) * BUF, tid);
+                tj.stash(oj, j0, k_lo + s * BK, k_hi, lds + (s & 1) * BUF + TI::kElems, tid);
                 __syncthreads();
             };
             if constexpr (ASYNC) {
@@ -477,13 +526,13 @@ dense_kernel(const DenseArgs<T> p) {
                 }
                 for (int64_t s = 0; s < whole; ++s) {
                     if (s + 1 < whole) copy(s + 1);
-                    step(ti, tj, lds + (s & 1) * BUF, c);
+                    step(ti, tj, lds + (s & 1) * BUF, c, BK);
                     landed();
                 }
                 if (whole < n_steps) {
                     through_regs(whole);
                     put(whole);
-                    step(ti, tj, lds + (whole & 1) * BUF, c);
+                    step(ti, tj, lds + (whole & 1) * BUF, c, k_hi - k_lo - whole * BK);
                     __syncthreads();
                 }
             } else {
@@ -493,7 +542,7 @@ dense_kernel(const DenseArgs<T> p) {
                 }
                 for (int64_t s = 0; s < n_steps; ++s) {
                     if (s + 1 < n_steps) through_regs(s + 1);
-                    step(ti, tj, lds + (s & 1) * BUF, c);
+                    step(ti, tj, lds + (s & 1) * BUF, c, k_hi - k_lo - s * BK);
                     if (s + 1 < n_steps) put(s + 1);
                     else __syncthreads();
                 }
@@ -544,7 +593,18 @@ dense_kernel(const DenseArgs<T> p) {
                 pair8(acc, pr, n, v);
                 if (j < p.j.n_out) store8<float>(part + j * p.i.n_out + i, v, p.i.n_out - i);
             }
-            if (my_sums && g == 0 && j < p.j.n_out) part[p.i.n_out * p.j.n_out + j] = sums[n][0];
+            if (SUM_MMA && my_sums && g == 0 && j < p.j.n_out) part[p.i.n_out * p.j.n_out + j] = sums[n][0];
+        }
+        if (SUM_ADD && my_sums) {
+            float *f = reinterpret_cast<float *>(lds);      // [thread][8]; behind the product's last barrier
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[8 * tid + e] = add_sums[e];
+            __syncthreads();
+            if (tid < BJ && j0 + tid < p.j.n_out) {
+                float v = 0.f;
+                for (int k = tid >> 3; k < THREADS; k += TJ::PER_ROW) v += f[8 * k + (tid & 7)];
+                part[p.i.n_out * p.j.n_out + j0 + tid] = v;
+            }
         }
     } else if constexpr (GATED) {
         with_act(p.act, [&](auto A) {
@@ -600,7 +660,10 @@ dense_kernel(const DenseArgs<T> p) {
                     float r[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) r[e] = 0.f;
-                    if (p.res) unpack8<T>(res[pr][n], r);
+                    if (p.res) {
+                        if (!inner && p.i.n_out >= 8) tail8_fix<T>(res[pr][n], p.i.n_out - i);
+                        unpack8<T>(res[pr][n], r);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float slope = 1.f;
@@ -711,7 +774,9 @@ static inline int dense_dw_slabs(int elem_bytes, int64_t rows, int64_t n, int64_
 // The tile of a product, by how many there would be: the chip takes part with as many CUs as there are tiles, and a larger tile reads less
 // LDS per operation and computes longer on what it has loaded.  (64 x 64: four waves of 64 x 16; 128 x 128: four of 64 x 64, two workgroups
 // to a CU; 256 x 256: eight of 128 x 64, one workgroup - gated backward, with its third accumulator, 256 x 192.)  65536 rows, 512 x 2048, bf16,
-// 256 against 128: gated forward 361 / 472 us, gated backward 728 / 843, input gradient 351 / 398, 2048 -> 512 152 / 180.
+// 256 against 128: gated forward 361 / 472 us, gated backward 728 / 843, input gradient 351 / 398, 2048 -> 512 152 / 180.  A short reduction
+// (below 256) is all epilogue, which only a second workgroup on the CU overlaps; a single step of it is all latency, which five small
+// workgroups hide better than two (20 -> 543, 129871 rows, bf16: 118 / 140 us).
 template <typename T, int MODE>
 static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
     constexpr bool GATED = MODE == kGatedFwd || MODE == kGatedBwd;
@@ -722,13 +787,16 @@ static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
         return ((reinterpret_cast<uintptr_t>(q.a) | reinterpret_cast<uintptr_t>(q.b)) & 15) == 0 && q.ld % 8 == 0 && (!tr || q.n_out % 8 == 0);
     };
     const bool async = sizeof(T) == 2 && aligned(p.i, TR_I) && aligned(p.j, TR_J) && (MODE != kGatedBwd || (aligned(p.i2, true) && aligned(p.j2, false)));
-    const bool wide = async && (MODE == kDenseDw ? dense_dw_wide(2, p.j.n_out, p.i.n_out) && count(256, 256) >= 128 : oi >= 256 && count(256, 256) >= 256);
-    const bool big = count(128, 128) >= 256;
+    const bool wide = async && (MODE == kDenseDw ? dense_dw_wide(2, p.j.n_out, p.i.n_out) && count(256, 256) >= 128
+                                                 : oi >= 256 && p.i.n_red >= 256 && count(256, 256) >= 256);
+    const bool one_step = (MODE == kDenseFwd || MODE == kDenseDz) && p.i.n_red <= 32;
+    const bool big = count(128, 128) >= 256 && !one_step;
     const int bi = wide ? 256 : big ? 128 : 64, bj = wide ? (MODE == kGatedBwd ? 192 : 256) : bi;
-    p.tiles_i = ceil_div<int64_t>(oi, bi);
-    p.tiles = count(bi, bj);
-    const int64_t grid = ceil_div<int64_t>(p.tiles, 8) * 8;
+    const int64_t grid = ceil_div<int64_t>(count(bi, bj), 8) * 8;
     if (grid > 0x7fffffff) return einval("dense: too many tiles for one launch");
+    p.tiles_i = (uint32_t)ceil_div<int64_t>(oi, bi);
+    p.tiles_j = (uint32_t)ceil_div<int64_t>(p.j.n_out, bj);
+    p.tiles = (uint32_t)count(bi, bj);
 #define ARCN_DK(WI_, WJ_, MI_, NJ_, A_) hipLaunchKernelGGL((dense_kernel<T, MODE, WI_, WJ_, MI_, NJ_, A_>), dim3((unsigned)grid), dim3(64 * WI_ * WJ_), 0, st, p)
     if constexpr (sizeof(T) == 2) {
         if (wide) ARCN_DK(2, 4, 8, (MODE == kGatedBwd ? 3 : 4), true);

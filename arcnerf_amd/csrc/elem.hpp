@@ -67,6 +67,30 @@ __device__ __forceinline__ void store16(T *p, u4v v) {
     *reinterpret_cast<u4v_any *>(p) = v;
 }
 
+// The same without a branch that waits: a row of at least VEC elements is read up to its LAST 16 bytes (`tail_at` moves the address there), and
+// what was loaded is shifted down to its place once it has arrived (`tail_fix`).  p: the pack's place in the row, left: elements of the row
+// from there on (any number).
+template <typename T>
+__device__ __forceinline__ const T *tail_at(const T *p, int64_t left) {
+    return left >= Elem<T>::VEC ? p : p + (left - Elem<T>::VEC);
+}
+template <typename T>
+__device__ __forceinline__ u4v tail_fix(u4v v, int64_t left) {
+    const int drop = left >= Elem<T>::VEC ? 0 : Elem<T>::VEC - (int)(left > 0 ? left : 0);   // elements in front of the pack
+    if (sizeof(T) == 2) {
+        if (drop & 8) v = u4v{0u, 0u, 0u, 0u};
+        if (drop & 4) v = u4v{v[2], v[3], 0u, 0u};
+        if (drop & 2) v = u4v{v[1], v[2], v[3], 0u};
+        if (drop & 1)
+            v = u4v{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+    } else {
+        if (drop & 4) v = u4v{0u, 0u, 0u, 0u};
+        if (drop & 2) v = u4v{v[2], v[3], 0u, 0u};
+        if (drop & 1) v = u4v{v[1], v[2], v[3], 0u};
+    }
+    return v;
+}
+
 // one 16-byte pack of a row of which `left` elements remain (<= 0: nothing is read); what lies behind the row's end reads as zero
 template <typename T>
 __device__ __forceinline__ u4v load_pack(const T *p, int64_t left) {

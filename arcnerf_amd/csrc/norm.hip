@@ -40,11 +40,49 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
     return v;
 }
 
-// the row's weight or bias (f32, or the rows' type), `fill` where the pointer is NULL or the row has ended
+// the lane's packs of a row (`rows` operands of one layout): a width that ends inside a pack is read by tail_at / tail_fix, rows narrower than a
+// pack element by element; `live` false: nothing is read
+template <typename T, int LPR, int NCH>
+__device__ __forceinline__ void load_row(const T *p, int lane, int C, bool live, u4v *r) {
+    if (C % Elem<T>::VEC == 0 || C < Elem<T>::VEC) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int col = (c * LPR + lane) * Elem<T>::VEC;
+            r[c] = load_pack(p + col, live ? C - col : 0);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int col = (c * LPR + lane) * Elem<T>::VEC;
+            r[c] = live ? load16(tail_at<T>(p + col, C - col)) : u4v{0u, 0u, 0u, 0u};
+        }
+    }
+}
+template <typename T, int LPR, int NCH>
+__device__ __forceinline__ void unpack_row(u4v *r, int lane, int C, float (*v)[Elem<T>::VEC]) {
+    const bool tail = C % Elem<T>::VEC != 0 && C >= Elem<T>::VEC;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        if (tail) r[c] = tail_fix<T>(r[c], C - (c * LPR + lane) * Elem<T>::VEC);
+        Elem<T>::unpack(r[c], v[c]);
+    }
+}
+
+// the lane's columns of the weight or bias (f32, or the rows' type), `fill` where the pointer is NULL or the row has ended
 template <typename T, typename WT>
 __device__ __forceinline__ void load_param(const WT *w, int col, int C, float fill, float *out) {
+    constexpr int V = Elem<T>::VEC, WV = Elem<WT>::VEC;
 #pragma unroll
-    for (int e = 0; e < Elem<T>::VEC; ++e) out[e] = (w && col + e < C) ? (float)w[col + e] : fill;
+    for (int e = 0; e < V; ++e) out[e] = fill;
+    if (!w || col >= C) return;
+    if (col + V <= C) {
+#pragma unroll
+        for (int h = 0; h < V / WV; ++h) Elem<WT>::unpack(load16(w + col + h * WV), out + h * WV);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (col + e < C) out[e] = (float)w[col + e];
+    }
 }
 
 template <typename T, typename WT, int LPR, int NCH>
@@ -66,11 +104,9 @@ layer_norm_fwd_kernel(const T *__restrict__ x, int64_t ld_x, const WT *__restric
         const int64_t r = r0 + sub;
         const bool live = r < rows;
         float v[NCH][VEC], s = 0.f;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int col = (c * LPR + lane) * VEC;
-            Elem<T>::unpack(load_pack(x + r * ld_x + col, live ? C - col : 0), v[c]);
-        }
+        u4v raw[NCH];
+        load_row<T, LPR, NCH>(x + r * ld_x, lane, C, live, raw);
+        unpack_row<T, LPR, NCH>(raw, lane, C, v);
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -114,12 +150,11 @@ layer_norm_bwd_kernel(const T *__restrict__ x, int64_t ld_x, const T *__restrict
         const bool live = r < rows;
         const float2 st = live ? stats[r] : make_float2(0.f, 0.f);
         float n[NCH][VEC], d[NCH][VEC], sg = 0.f, sgn = 0.f;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int col = (c * LPR + lane) * VEC;
-            Elem<T>::unpack(load_pack(x + r * ld_x + col, live ? C - col : 0), n[c]);
-            Elem<T>::unpack(load_pack(dy + r * ld_dy + col, live ? C - col : 0), d[c]);
-        }
+        u4v raw_x[NCH], raw_dy[NCH];
+        load_row<T, LPR, NCH>(x + r * ld_x, lane, C, live, raw_x);
+        load_row<T, LPR, NCH>(dy + r * ld_dy, lane, C, live, raw_dy);
+        unpack_row<T, LPR, NCH>(raw_x, lane, C, n);
+        unpack_row<T, LPR, NCH>(raw_dy, lane, C, d);
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
