@@ -26,12 +26,12 @@ ARCN_EXPORT int arcn_dense_fwd(const void *x, int64_t ld_x, const void *w, const
     return ARCN_DENSE_DISPATCH(fwd(x, ld_x, w, bias, residual, ld_res, y, act, beta, n_rows, K, N, as_stream(stream)));
 }
 
-ARCN_EXPORT int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, int dtype, int act, float beta,
-                              int64_t n_rows, int K, int N, void *stream) {
+ARCN_EXPORT int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, void *dx, int dtype, int act,
+                              float beta, int64_t n_rows, int K, int N, void *stream) {
     if (!dense_type(dtype) || !dense_act(act, beta) || !dense_sizes(n_rows, K, N)) return einval("dense_dz: unsupported type, activation or size");
     if (n_rows == 0) return ARCN_OK;
     if (!x || !w || !dy || !dz || ld_x < K || ld_dy < N) return einval("dense_dz: missing / invalid argument");
-    return ARCN_DENSE_DISPATCH(dz(x, ld_x, w, bias, dy, ld_dy, dz, act, beta, n_rows, K, N, as_stream(stream)));
+    return ARCN_DENSE_DISPATCH(dz_dx(x, ld_x, w, bias, dy, ld_dy, dz, dx, act, beta, n_rows, K, N, as_stream(stream)));
 }
 
 ARCN_EXPORT int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int dtype, int64_t n_rows, int N, int K, void *stream) {

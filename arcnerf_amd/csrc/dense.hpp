@@ -11,7 +11,8 @@
 // Nothing of the forward pass but its inputs (and h) is kept for the backward: a pre-activation is computed again in the tile that needs
 // its slope, in f32, where a saved one would have been rounded to the layer's type and cost its bytes twice (2 K operations per 4 bytes:
 // at K = 256 a tile computes it faster than HBM would return it).  The gated backward computes g, u AND dh of a tile in registers; only
-// dg and du, each rounded once, are written.
+// dg and du, each rounded once, are written.  (That rounding, and h's, are the 16-bit types' only ones between a call's inputs and its
+// results: dx, dW and the bias sums are made from the rounded values, which costs them as much again as their own rounding, 1.4 x in all.)
 //
 // f32 operands are split into three bf16 planes on their way into LDS, x = hi + mid + lo, and six products (hi hi, hi mid, mid hi, hi lo,
 // lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  416 TFLOP/s of f32-accurate products against 157
@@ -371,6 +372,8 @@ struct DenseArgs {
     int64_t ld_res;
     T *out;
     int64_t ld_out;
+    T *out2;                 // dense_dz_dx_kernel: dx
+    int64_t ld_out2;
     float *partial;          // kDenseDw: [slab][n_j * n_i (+ n_j column sums of j)]
     int want_sums;
     int act;
@@ -382,6 +385,16 @@ struct DenseArgs {
 // blockIdx -> tile: workgroups are dealt to the 8 XCDs in turn, so each XCD gets a contiguous range of tiles and the tiles that share
 // their J rows (the large operand) meet in one L2
 __device__ __forceinline__ uint32_t xcd_tile() { return (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
+
+// the 8 consecutive features that a lane ends up with of a pair of MFMA tiles (every lane takes part)
+__device__ __forceinline__ void swap8(f4v a, f4v b, float *v) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const auto sw = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, (float)a[r]), __builtin_bit_cast(uint32_t, (float)b[r]), false, false);
+        v[r] = __builtin_bit_cast(float, (uint32_t)sw[0]);
+        v[4 + r] = __builtin_bit_cast(float, (uint32_t)sw[1]);
+    }
+}
 
 // ASYNC: operands straight from memory to LDS (Tile::copy; launch_tiles checks what it needs)
 template <typename T, int MODE, int WI, int WJ, int MI, int NJ, bool ASYNC>
@@ -567,15 +580,7 @@ dense_kernel(const DenseArgs<T> p) {
     }
 
     // ---- epilogue -----------------------------------------------------------------------------------------------------------------------
-    auto pair8 = [&](auto &c, int pr, int n, float *v) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const auto sw = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, (float)c[2 * pr][n][r]),
-                                                             __builtin_bit_cast(uint32_t, (float)c[2 * pr + 1][n][r]), false, false);
-            v[r] = __builtin_bit_cast(float, (uint32_t)sw[0]);
-            v[4 + r] = __builtin_bit_cast(float, (uint32_t)sw[1]);
-        }
-    };
+    auto pair8 = [&](auto &c, int pr, int n, float *v) { swap8(c[2 * pr][n], c[2 * pr + 1][n], v); };
     auto bias8 = [&](const T *b, int64_t i, float *v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
@@ -684,21 +689,22 @@ dense_kernel(const DenseArgs<T> p) {
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------------------
 // A handful of rows leaves the tiles above with a few workgroups that wait on memory.  Here a workgroup makes 16 features (gated: 16 of
-// both matrices) of all rows, its four waves share the reduction in steps of 32 and read their operands straight into fragments; the
-// partial sums meet in LDS.  The weights are read once, by n_i / 16 workgroups at a time.
+// both matrices) of up to 32 rows, its four waves share the reduction in steps of 32 and read their operands straight into fragments; the
+// partial sums meet in LDS.  The weights are read once per 32 rows, by n_i / 16 workgroups.
+// One row, 1024 x 1024 bf16: 3.5 us, 2 MB of weight.
 template <typename T, bool GATED, int NJ>
 __global__ void __launch_bounds__(256)
 dense_few_kernel(const DenseArgs<T> p) {
     constexpr int P = Mma<T>::P, NG = GATED ? 2 : 1;
     __shared__ float lds[4][NG * NJ][16][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, o = lane & 15, g = lane >> 4;
-    const int64_t i0 = (int64_t)blockIdx.x * 16, K = p.i.n_red;
+    const int64_t i0 = (int64_t)blockIdx.x * 16, j0 = (int64_t)blockIdx.y * 16 * NJ, K = p.i.n_red;
     const int64_t iw = i0 + o < p.i.n_out ? i0 + o : p.i.n_out - 1;
     const T *wp[2] = {p.i.a + iw * p.i.ld, GATED ? p.i.b + iw * p.i.ld : nullptr};
     const T *xp[NJ];
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
-        const int64_t j = 16 * n + o;
+        const int64_t j = j0 + 16 * n + o;
         xp[n] = p.j.a + (j < p.j.n_out ? j : p.j.n_out - 1) * p.j.ld;
     }
     f4v acc[NG][NJ];
@@ -737,7 +743,7 @@ dense_few_kernel(const DenseArgs<T> p) {
     if (i >= p.i.n_out) return;
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
-        const int64_t j = 16 * n + lj;
+        const int64_t j = j0 + 16 * n + lj;
         if (j >= p.j.n_out) break;
         float v[NG];
 #pragma unroll
@@ -754,8 +760,167 @@ dense_few_kernel(const DenseArgs<T> p) {
     }
 }
 
+// ---- a weight that stays in LDS: dz and dx in one kernel -----------------------------------------------------------------------------------
+// The backward of a layer whose whole weight fits LDS (16-bit types, up to 128 inputs and 512 outputs: 128 KB) moves 8 bytes per 4 K operations:
+// it is bound by HBM, and as two products dz alone goes out and comes back.  Here a workgroup loads the weight once and its waves run on
+// their own, 16 rows at a time, without another barrier.  A lane's fragments of x come straight from memory (its row's 16 bytes); the
+// pre-activation is computed again for 128 features at a time, and because a lane's 8 consecutive features of dz are what the next
+// product wants as its J fragment, dx = dz W follows in registers on the SAME weight, read the other way round (transposing reads).  The
+// reduction over features is dealt to the lanes as the features fell (f8).  x and dy in, dz and dx out: 128 -> 112, 317560 rows, bf16 77 us
+// (3.9 TB/s) against 67 + 47 as two products.  (With 256 inputs the accumulators of dx do not fit beside the rest: 236 us against 127 + 75.)
+template <typename T, int KS>
+__global__ void __launch_bounds__(512, 2)
+dense_dz_dx_kernel(const DenseArgs<T> p) {
+    constexpr int WAVES = 8, NT = 8, ROW = KS * 4;      // NT: feature tiles of a pass; ROW: 16-byte chunks per LDS row
+    extern __shared__ __attribute__((aligned(16))) short w[];      // [N up to a multiple of 128][KS * 32], then the bias
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, o = lane & 15, g = lane >> 4, f8 = 16 * (g & 1) + 8 * (g >> 1);
+    int K = (int)p.i.n_red, N = (int)p.i.n_out;
+    const int ks = (K + 31) / 32, n_pad = (N + 127) / 128 * 128;
+    T *bias = reinterpret_cast<T *>(w + n_pad * ROW * 8);
+    // chunk c of row n at c ^ swizzle(n): 8 rows of one chunk, and 4 rows of two, fall on different banks
+    auto swizzle = [](int n) { return ((n & 3) << 1) | ((n >> 2) & 1); };
+    for (int q = tid; q < n_pad * ROW; q += 64 * WAVES) {
+        const int n = q / ROW, c = q % ROW;
+        *reinterpret_cast<u4v *>(w + 8 * (n * ROW + (c ^ swizzle(n)))) = load8<T>(p.i.a + (int64_t)(n < N ? n : 0) * p.i.ld + 8 * c, n < N ? K - 8 * c : 0).v[0];
+    }
+    for (int n = tid; n < n_pad; n += 64 * WAVES) bias[n] = p.bias && n < N ? p.bias[n] : (T)0.f;
+    __syncthreads();
+
+    const int64_t rows = p.j.n_out, step = (int64_t)gridDim.x * WAVES * 16;
+    u4v x[KS];
+    auto fetch = [&](int64_t r) {
+        const T *row = p.j.a + (r + o < rows ? r + o : rows - 1) * p.j.ld;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+            if (kk < ks) x[kk] = load16(tail_at<T>(row + 32 * kk + 8 * g, K - 32 * kk - 8 * g));
+    };
+    int64_t r0 = ((int64_t)blockIdx.x * WAVES + wave) * 16;
+    if (r0 < rows) fetch(r0);
+    for (; r0 < rows; r0 += step) {
+        const int64_t r = r0 + o < rows ? r0 + o : rows - 1;
+        const bool live = r0 + o < rows;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+            if (kk < ks && 32 * kk + 32 > K) x[kk] = tail_fix<T>(x[kk], K - 32 * kk - 8 * g);
+        f4v dx[2 * KS];
+#pragma unroll
+        for (int m = 0; m < 2 * KS; ++m) dx[m] = f4v{0.f, 0.f, 0.f, 0.f};
+        for (int n0 = 0; n0 < n_pad; n0 += 128) {
+            // What the loops could keep they must not: weight and bias are read again for every group, the masks of the last columns and the
+            // addresses of the weight's fragments (a few per lane, everything else is in the instructions' offsets) are computed again:
+            // hundreds of registers.
+            asm volatile("" : "+s"(K), "+s"(N) : : "memory");
+            uint32_t af[2], at[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                af[h] = 16 * ((n0 + o) * ROW + ((4 * h + g) ^ swizzle(o)));      // row o, chunk 4 h + g
+                asm volatile("" : "+v"(af[h]));
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {      // row f8 + 4 h + o / 4, column 16 m + 4 (o % 4)
+                    at[h][m] = 16 * ((n0 + f8 + 4 * h + (o >> 2)) * ROW + 2 * (m ^ (o >> 2)) + (((o >> 1) & 1) ^ h)) + 8 * (o & 1);
+                    asm volatile("" : "+v"(at[h][m]));
+                }
+            }
+            const char *const wb = reinterpret_cast<const char *>(w);
+            u4v dy[NT / 2];
+#pragma unroll
+            for (int pr = 0; pr < NT / 2; ++pr) dy[pr] = load16(tail_at<T>(p.res + r * p.ld_res + n0 + 32 * pr + f8, N - n0 - 32 * pr - f8));
+            f4v z[NT];
+#pragma unroll
+            for (int m = 0; m < NT; ++m) z[m] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                if (kk >= ks) break;
+                const s8v b = __builtin_bit_cast(s8v, x[kk]);
+#pragma unroll
+                for (int m = 0; m < NT; ++m) {
+                    const s8v a = *reinterpret_cast<const s8v *>(wb + af[kk & 1] + 16 * m * ROW * 16 + (kk >> 1) * 128);
+                    z[m] = Mma<T>::mma(&a, &b, z[m], 1.f);
+                }
+            }
+            if (n0 + 128 >= n_pad && r0 + step < rows) fetch(r0 + step);      // the next rows', behind the rest of this group
+            with_act(p.act, [&](auto A) {
+#pragma unroll
+                for (int pr = 0; pr < NT / 2; ++pr) {
+                    float v[8], b[8], q[8];
+                    swap8(z[2 * pr], z[2 * pr + 1], v);
+                    Elem<T>::unpack(*reinterpret_cast<const u4v *>(bias + n0 + 32 * pr + f8), b);
+                    if (n0 + 32 * pr + 32 > N) dy[pr] = tail_fix<T>(dy[pr], N - n0 - 32 * pr - f8);
+                    Elem<T>::unpack(dy[pr], q);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float slope;
+                        act_eval<A(), true, true>(v[e] + b[e], p.beta, p.inv_beta, slope);
+                        v[e] = q[e] * slope;
+                    }
+                    dy[pr] = Elem<T>::pack(v);      // dz from here on
+                }
+            });
+#pragma unroll
+            for (int pr = 0; pr < NT / 2; ++pr) {
+                const int i = n0 + 32 * pr + f8;
+                if (N % 32 == 0) {
+                    if (live && i < N) store16(p.out + r * p.ld_out + i, dy[pr]);
+                } else {
+                    store_pack(p.out + r * p.ld_out + i, dy[pr], live ? N - i : 0);
+                }
+            }
+#pragma unroll
+            for (int pr = 0; pr < NT / 2; ++pr) {
+                if (n0 + 32 * pr >= N) break;
+                const s8v b = __builtin_bit_cast(s8v, dy[pr]);
+#pragma unroll
+                for (int m = 0; m < 2 * KS; ++m) {
+                    s4v h[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s4v *)(wb + at[e][m & 3] + 32 * pr * ROW * 16 + (m >> 2) * 128));
+                    const s8v a = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    dx[m] = Mma<T>::mma(&a, &b, dx[m], 1.f);
+                }
+            }
+        }
+#pragma unroll
+        for (int pr = 0; pr < KS; ++pr) {
+            if (pr >= ks) break;
+            const int i = 32 * pr + f8;
+            float v[8];
+            swap8(dx[2 * pr], dx[2 * pr + 1], v);
+            if (K % 32 == 0) {
+                if (live) store16(p.out2 + r * p.ld_out2 + i, Elem<T>::pack(v));
+            } else {
+                store_pack(p.out2 + r * p.ld_out2 + i, Elem<T>::pack(v), live ? K - i : 0);
+            }
+        }
+    }
+}
+
 // ---- launches -------------------------------------------------------------------------------------------------------------------------
-constexpr int64_t kFewRows = 32;
+// dense_few_kernel: as long as two of its workgroups to a CU (f32: eight) do the product.  One feature block of it costs 3 - 5 us whatever the
+// rows, the tiles' first step waits longer and in f32 computes six products on a few CUs: 256 x 256 bf16 3.5 us at 512 rows (tiles 4.4), f32
+// 4.7 (11.1); 1024 x 1024 bf16 5.3 at 128 rows and 13.2 at 512 (7.9), f32 8.6 and 24 (34).
+static inline bool dense_few(int elem_bytes, int64_t rows, int64_t n) {
+    return rows <= 1024 && ceil_div<int64_t>(n, 16) * ceil_div<int64_t>(rows, 32) <= (elem_bytes == 2 ? 512 : 2048);
+}
+
+
+// dense_dz_dx_kernel's layers: 16 bits, enough rows for the weight that every CU loads first
+// (16384 rows: 63 -> 40, 20000 rows 13 us against 9 + 9 of which one launch is 3)
+constexpr int64_t kStayRows = 16384;
+template <typename T>
+static bool dense_stays(int64_t rows, int K, int N) {
+    return sizeof(T) == 2 && K >= 8 && N >= 8 && K <= 128 && N <= 512 && rows >= kStayRows;
+}
+template <typename T>
+static int launch_dz_dx(const DenseArgs<T> &p, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        const int bytes = ceil_div<int>((int)p.i.n_out, 128) * 128 * (256 + 2);      // the weight's rows of 128 inputs, and the bias
+        const int64_t g = ceil_div<int64_t>(p.j.n_out, 128), most = bytes <= 80 * 1024 ? 512 : 256;
+        hipLaunchKernelGGL((dense_dz_dx_kernel<T, 4>), dim3((unsigned)(g < most ? g : most)), dim3(512), bytes, st, p);
+    }
+    return check_launch("dense_dz");
+}
 
 // slabs of a weight gradient: the rows are cut so that tiles times slabs fill the chip (256 x 256 tiles: once; 128 x 128: two workgroups to a
 // CU), none shorter than 256 rows.  A rule on sizes and type only: the scratch a caller brings is as large whatever its pointers' alignment.
@@ -818,6 +983,8 @@ struct DenseOps {
     static int dz(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, int act, float beta, int64_t rows, int K, int N,
                   hipStream_t st);
     static int dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int64_t rows, int N, int K, hipStream_t st);
+    static int dz_dx(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, void *dx, int act, float beta, int64_t rows, int K,
+                     int N, hipStream_t st);
     static int dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, float *scratch, int64_t rows, int N, int K, hipStream_t st);
     static int gated_fwd(const void *x, int64_t ld_x, const void *wg, const void *wu, const void *bg, const void *bu, void *h, int act, float beta, int64_t rows, int K,
                          int H, hipStream_t st);

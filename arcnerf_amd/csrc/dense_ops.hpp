@@ -24,8 +24,8 @@ int DenseOps<T>::fwd(const void *x, int64_t ld_x, const void *w, const void *b, 
     p.act = act;
     p.beta = beta;
     p.inv_beta = 1.f / beta;
-    if (rows <= kFewRows) {
-        const dim3 grid((unsigned)ceil_div<int>(N, 16));
+    if (dense_few(sizeof(T), rows, N)) {
+        const dim3 grid((unsigned)ceil_div<int>(N, 16), (unsigned)ceil_div<int64_t>(rows, 32));
         if (rows <= 16) hipLaunchKernelGGL((dense_few_kernel<T, false, 1>), grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((dense_few_kernel<T, false, 2>), grid, dim3(256), 0, st, p);
         return check_launch("dense_fwd");
@@ -61,6 +61,29 @@ int DenseOps<T>::dx(const void *dz, int64_t ld_dz, const void *w, const void *w2
 }
 
 template <typename T>
+int DenseOps<T>::dz_dx(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz_, void *dx_, int act, float beta, int64_t rows,
+                       int K, int N, hipStream_t st) {
+    if (!dx_ || !dense_stays<T>(rows, K, N)) {
+        if (int rc = dz(x, ld_x, w, b, dy, ld_dy, dz_, act, beta, rows, K, N, st)) return rc;
+        return dx_ ? dx(dz_, N, w, nullptr, dx_, rows, N, K, st) : ARCN_OK;
+    }
+    DenseArgs<T> p = {};
+    p.i = {tp<T>(w), nullptr, K, N, K, 0};
+    p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
+    p.bias = tp<T>(b);
+    p.res = tp<T>(dy);
+    p.ld_res = ld_dy;
+    p.out = static_cast<T *>(dz_);
+    p.ld_out = N;
+    p.out2 = static_cast<T *>(dx_);
+    p.ld_out2 = K;
+    p.act = act;
+    p.beta = beta;
+    p.inv_beta = 1.f / beta;
+    return launch_dz_dx<T>(p, st);
+}
+
+template <typename T>
 int DenseOps<T>::dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, float *scratch, int64_t rows, int N, int K, hipStream_t st) {
     DenseArgs<T> p = {};
     p.i = {tp<T>(x), nullptr, ld_x, K, rows, 0};
@@ -87,8 +110,8 @@ int DenseOps<T>::gated_fwd(const void *x, int64_t ld_x, const void *wg, const vo
     p.act = act;
     p.beta = beta;
     p.inv_beta = 1.f / beta;
-    if (rows <= kFewRows) {
-        const dim3 grid((unsigned)ceil_div<int>(H, 16));
+    if (dense_few(sizeof(T), rows, 2 * (int64_t)H)) {
+        const dim3 grid((unsigned)ceil_div<int>(H, 16), (unsigned)ceil_div<int64_t>(rows, 32));
         if (rows <= 16) hipLaunchKernelGGL((dense_few_kernel<T, true, 1>), grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((dense_few_kernel<T, true, 2>), grid, dim3(256), 0, st, p);
         return check_launch("gated_fwd");

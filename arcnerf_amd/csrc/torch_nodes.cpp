@@ -56,7 +56,7 @@ struct Rows {
 };
 Rows rows_of(const char *name, const Tensor &t, int64_t width, const Tensor &like) {
     TORCH_CHECK(t.is_cuda(), "arcnerf_amd ops run on the GPU only (got a ", t.device(), " ", name, "); there is no CPU fallback");
-    TORCH_CHECK(t.dim() >= 1 && t.size(-1) == width && width >= 1, "arcnerf_amd: ", name, " must be (..., ", width, "), got ", t.sizes());
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) == width && width >= 1 && width <= (1 << 24), "arcnerf_amd: ", name, " must be (..., ", width, "), got ", t.sizes());
     TORCH_CHECK(t.scalar_type() == like.scalar_type() && t.device() == like.device(), "arcnerf_amd: ", name, " is ", t.scalar_type(), " on ", t.device(),
                 ", not ", like.scalar_type(), " on ", like.device());
     Rows r;
@@ -89,7 +89,7 @@ void check_like(const char *name, const Tensor &t, at::IntArrayRef shape) {
 
 std::vector<int64_t> with_last(const Tensor &x, int64_t n) {
     std::vector<int64_t> s = x.sizes().vec();
-    TORCH_CHECK(!s.empty(), "arcnerf_amd: x must be (..., width), got a scalar");
+    TORCH_CHECK(!s.empty() && n <= (1 << 24), "arcnerf_amd: x must be (..., width) and a width at most 2^24, got ", x.sizes(), " and ", n);
     s.back() = n;
     return s;
 }
@@ -255,11 +255,11 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
                 const Tensor bc = b.defined() ? b.contiguous() : b;
                 dz.t = fresh({r.n, N}, x);
                 dz.ld = N;
-                call(arcn_dense_dz(r.p(), r.ld, ptr(w), ptr(bc), dy.p(), dy.ld, dz.t.data_ptr(), dt, (int)act, (float)ctx->saved_data["beta"].toDouble(), r.n,
-                                   (int)K, (int)N, go.stream),
+                if (want_dx) out[0] = fresh(x.sizes(), x);
+                call(arcn_dense_dz(r.p(), r.ld, ptr(w), ptr(bc), dy.p(), dy.ld, dz.t.data_ptr(), out_ptr(out[0]), dt, (int)act,
+                                   (float)ctx->saved_data["beta"].toDouble(), r.n, (int)K, (int)N, go.stream),
                      "dense_dz");
-            }
-            if (want_dx) {
+            } else if (want_dx) {
                 out[0] = fresh(x.sizes(), x);
                 call(arcn_dense_dx(dz.p(), dz.ld, ptr(w), nullptr, out[0].data_ptr(), dt, r.n, (int)N, (int)K, go.stream), "dense_dx");
             }

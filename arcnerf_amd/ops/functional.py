@@ -1293,20 +1293,21 @@ def dense_fwd(x, w, bias=None, residual=None, act=None, beta=1.0):
     return y
 
 
-def dense_dz(x, w, bias, dy, act, beta=1.0):
-    """dy * act'(x @ w.T + bias), the pre-activation computed again; dy itself where there is no activation"""
+def dense_dz(x, w, bias, dy, act, beta=1.0, want_dx=False):
+    """dy * act'(x @ w.T + bias), the pre-activation computed again (dy itself where there is no activation); want_dx: also that @ w"""
     _req(x, w, bias, dy)
     x, ld = _ffn_rows('x', x)
     (S, K), Nn, code = x.shape, w.shape[0], _dense_act(act, beta)
     w, bias = _ffn_param('weight', w, (Nn, K), x), _ffn_param('bias', bias, (Nn,), x)
     dy, ld_dy = _ffn_rows('dy', dy, Nn, like=x)
     if code == 0:
-        return dy
+        return (dy, dense_dx(dy, w)) if want_dx else dy
     dz = _fresh((S, Nn), x.dtype, x.device)
+    dx = _fresh((S, K), x.dtype, x.device) if want_dx else None
     with _device_of(x):
-        N.check(N.lib().arcn_dense_dz(x.data_ptr(), ld, N.ptr(w), N.ptr(bias), dy.data_ptr(), ld_dy, N.ptr(dz), _DTYPE[x.dtype], code, float(beta), S, K, Nn,
+        N.check(N.lib().arcn_dense_dz(x.data_ptr(), ld, N.ptr(w), N.ptr(bias), dy.data_ptr(), ld_dy, N.ptr(dz), N.ptr(dx), _DTYPE[x.dtype], code, float(beta), S, K, Nn,
                                       N.stream()), 'dense_dz')
-    return dz
+    return (dz, dx) if want_dx else dz
 
 
 def dense_dx(dz, w, w2=None):

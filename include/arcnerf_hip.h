@@ -833,9 +833,10 @@ int arcn_layer_norm_bwd(const void *x, int64_t ld_x, const void *dy, int64_t ld_
  * (f32 accuracy; infinities and NaN give NaN). */
 int arcn_dense_fwd(const void *x, int64_t ld_x, const void *w, const void *bias, const void *residual, int64_t ld_res, void *y, int dtype, int act,
                    float beta, int64_t n_rows, int K, int N, void *stream);
-/* dz (n_rows, N) = dy act'(x w^T + bias): the gradient of the pre-activation, which is computed again from x (nothing was saved) */
-int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, int dtype, int act, float beta,
-                  int64_t n_rows, int K, int N, void *stream);
+/* dz (n_rows, N) = dy act'(x w^T + bias): the gradient of the pre-activation, which is computed again from x (nothing was saved); unless dx is
+ * NULL also dx (n_rows, K) = dz w, in the same kernel where the weight fits on chip */
+int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, void *dx, int dtype, int act,
+                  float beta, int64_t n_rows, int K, int N, void *stream);
 /* dx (n_rows, K) = dz (n_rows, N) w (N, K).  w2 not NULL (N even): the weight's first N / 2 rows are w (N / 2, K), the others w2. */
 int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int dtype, int64_t n_rows, int N, int K, void *stream);
 /* dw (N, K) = dz^T x and, unless db is NULL, db (N) = the column sums of dz.  scratch: arcn_dense_dw_scratch_floats floats. */

@@ -98,7 +98,7 @@ def test_entry_points_refuse_before_a_launch(lib):
     assert lib.arcn_dense_fwd(p, 8, p, n, n, 0, p, 0, 0, 1.0, -1, 8, 8, n) == -1
     assert lib.arcn_dense_fwd(n, 8, n, n, n, 0, n, 2, 8, 1.0, 0, 8, 8, n) == 0
     assert b'dense_fwd' in lib.arcn_last_error()
-    assert lib.arcn_dense_dz(p, 8, p, n, n, 8, p, 0, 1, 1.0, 4, 8, 8, n) == -1
+    assert lib.arcn_dense_dz(p, 8, p, n, n, 8, p, p, 0, 1, 1.0, 4, 8, 8, n) == -1
     assert lib.arcn_dense_dx(p, 7, p, p, p, 0, 4, 7, 8, n) == -1                                  # two halves of an odd width
     assert lib.arcn_dense_dw_scratch_floats(1000, 64, 32, 0) >= 64 * 33
     assert lib.arcn_dense_dw_scratch_floats(1000, 64, 32, 9) == 0

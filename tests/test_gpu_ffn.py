@@ -205,7 +205,7 @@ def check_dense(rows, k, n, dtype, act, beta=1.0, pitch=0, bias=True, residual=T
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
-@pytest.mark.parametrize('rows,k,n,pitch', [(1, 1, 1, 0), (1, 256, 256, 0), (2, 31, 17, 1), (16, 32, 16, 0), (17, 33, 15, 0), (32, 520, 70, 3), (33, 8, 8, 0), (33, 64, 64, 0),
+@pytest.mark.parametrize('rows,k,n,pitch', [(1, 1, 1, 0), (1, 256, 256, 0), (2, 31, 17, 1), (16, 32, 16, 0), (17, 33, 15, 0), (32, 520, 70, 3), (33, 8, 8, 0), (33, 64, 64, 0), (65, 100, 1030, 0), (999, 40, 48, 1),
                                             (40, 96, 200, 0), (130, 283, 131, 5), (257, 319, 129, 2), (1000, 7, 3, 0)])
 def test_dense_sizes(dtype, rows, k, n, pitch):
     check_dense(rows, k, n, dtype, 'silu', pitch=pitch)
@@ -216,6 +216,14 @@ def test_dense_large_tiles(dtype):
     """enough tiles for the 128 x 128 kernels of all three products, none of them whole"""
     check_dense(33001, 129, 130, dtype, 'gelu')
     check_dense(16500, 264, 136, dtype, None, pitch=8)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,n,act,pitch', [(16384, 8, 8, 'silu', 0), (16401, 128, 128, 'gelu', 0), (20000, 100, 60, 'softplus', 3), (17000, 256, 256, 'silu', 0),
+                                                (16999, 250, 13, 'sigmoid', 1), (40007, 33, 256, 'gelu', 0), (70001, 63, 31, None, 0), (33001, 9, 129, 'relu', 5)])
+def test_dense_small_layer_many_rows(dtype, rows, k, n, act, pitch):
+    """layers whose weight stays on chip (16-bit types), every wave with several groups of rows and a last partial one"""
+    check_dense(rows, k, n, dtype, act, pitch=pitch, bias=act != 'silu', residual=act != 'sigmoid')
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
@@ -372,7 +380,7 @@ def check_gated(rows, k, hid, n, dtype, act='silu', beta=1.0, pitch=0, bias=True
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
-@pytest.mark.parametrize('rows,k,hid,n,pitch', [(1, 1, 1, 1, 0), (1, 256, 1024, 256, 0), (8, 64, 96, 64, 0), (17, 33, 31, 29, 1), (32, 40, 65, 40, 0), (33, 32, 32, 32, 0),
+@pytest.mark.parametrize('rows,k,hid,n,pitch', [(1, 1, 1, 1, 0), (1, 256, 1024, 256, 0), (8, 64, 96, 64, 0), (17, 33, 31, 29, 1), (32, 40, 65, 40, 0), (33, 32, 32, 32, 0), (100, 20, 1100, 20, 0), (1024, 24, 40, 16, 0),
                                                 (61, 131, 347, 131, 3), (300, 48, 130, 24, 0), (129, 72, 64, 200, 8)])
 def test_gated_sizes(dtype, rows, k, hid, n, pitch):
     check_gated(rows, k, hid, n, dtype, pitch=pitch)
