@@ -853,6 +853,10 @@ dense_dz_dx_kernel(const DenseArgs<T> p) {
                         act_eval<A(), true, true>(v[e] + b[e], p.beta, p.inv_beta, slope);
                         v[e] = q[e] * slope;
                     }
+                    if (n0 + 32 * pr + 32 > N) {      // features behind the last: zero, whatever an infinity in x made of their slope
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = n0 + 32 * pr + f8 + e < N ? v[e] : 0.f;
+                    }
                     dy[pr] = Elem<T>::pack(v);      // dz from here on
                 }
             });

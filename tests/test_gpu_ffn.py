@@ -220,7 +220,7 @@ def test_dense_large_tiles(dtype):
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
 @pytest.mark.parametrize('rows,k,n,act,pitch', [(16384, 8, 8, 'silu', 0), (16401, 128, 128, 'gelu', 0), (20000, 100, 60, 'softplus', 3), (17000, 256, 256, 'silu', 0),
-                                                (16999, 250, 13, 'sigmoid', 1), (40007, 33, 256, 'gelu', 0), (70001, 63, 31, None, 0), (33001, 9, 129, 'relu', 5)])
+                                                (16999, 250, 13, 'sigmoid', 1), (40007, 33, 256, 'gelu', 0), (16400, 128, 512, 'silu', 0), (70001, 63, 31, None, 0), (33001, 9, 129, 'relu', 5)])
 def test_dense_small_layer_many_rows(dtype, rows, k, n, act, pitch):
     """layers whose weight stays on chip (16-bit types), every wave with several groups of rows and a last partial one"""
     check_dense(rows, k, n, dtype, act, pitch=pitch, bias=act != 'silu', residual=act != 'sigmoid')
@@ -231,6 +231,24 @@ def test_dense_small_layer_many_rows(dtype, rows, k, n, act, pitch):
 def test_dense_activations(dtype, act, beta):
     check_dense(77, 40, 50, dtype, act, beta)
     check_dense(9, 40, 50, dtype, act, beta, bias=False, residual=False)
+
+
+@pytest.mark.parametrize('rows', [200, 16400])
+def test_dense_infinite_input_stays_in_its_row(rows):
+    """an infinity in one input row: its pre-activations are infinite and the slopes zero, every other row is as without it"""
+    from arcnerf_amd.ops import autograd as A
+    x, w, b, _, dy = (t.cuda() for t in dense_inputs(rows, 24, 13, torch.bfloat16))
+    bad = x.clone()
+    bad[5, 3] = float('inf')
+    w[:, 3] = w[:, 3].abs() + 0.25
+    got = []
+    for t in (x, bad):
+        t = t.requires_grad_(True)
+        y = A.linear_act_residual(t, w, b, act='sigmoid')
+        got.append((y.detach(), torch.autograd.grad(y, t, dy)[0]))
+    keep = torch.arange(rows, device='cuda') != 5
+    assert torch.equal(got[0][0][keep], got[1][0][keep]) and torch.equal(got[0][1][keep], got[1][1][keep])
+    assert (got[1][0][5] == 1).all() and (got[1][1][5] == 0).all()
 
 
 def test_dense_far_preactivations():
