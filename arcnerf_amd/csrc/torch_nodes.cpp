@@ -7,6 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <cstdlib>
@@ -101,19 +102,17 @@ struct Launch {
     explicit Launch(const Tensor &t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-// first order only: where a graph of the gradients is asked for, differentiating them raises
-tensor_list first_order(tensor_list grads, bool graph, const char *what) {
+// First order only: where a graph of the gradients is asked for they hang on a node that raises.  Its edges lead to everything that the
+// gradients depend on (`from`: what the node saved and the gradient that came in), so that a differentiation which asks for any of these
+// runs it, also one with other paths to them (a loss that has terms in both the result and its gradient, a list of inputs).
+tensor_list first_order(tensor_list grads, bool graph, const char *what, const tensor_list &from) {
     if (!graph) return grads;
-    std::vector<size_t> at;
-    tensor_list some;
-    for (size_t k = 0; k < grads.size(); ++k)
-        if (grads[k].defined()) {
-            at.push_back(k);
-            some.push_back(grads[k].detach().requires_grad_(true));
+    auto err = std::make_shared<torch::autograd::Error>(std::string("arcnerf_amd: ") + what + " can be differentiated once only", torch::autograd::collect_next_edges(from));
+    for (Tensor &g : grads)
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::set_history(g, err);
         }
-    auto err = std::make_shared<torch::autograd::DelayedError>(std::string("arcnerf_amd: ") + what + " can be differentiated once only", (int64_t)some.size());
-    some = (*err)(std::move(some));
-    for (size_t k = 0; k < at.size(); ++k) grads[at[k]] = some[k];
     return grads;
 }
 
@@ -182,7 +181,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (r.n == 0) {
             for (int k : {1, 2})
                 if (out[k].defined()) out[k].zero_();
-            return first_order(std::move(out), graph, "layer_norm");
+            return first_order(std::move(out), graph, "layer_norm", {x, w, g[0]});
         }
         const int dt = type_code(x, "x");
         const Tensor wc = w.defined() ? w.contiguous() : w;
@@ -192,7 +191,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         call(arcn_layer_norm_bwd(r.p(), r.ld, dy.p(), dy.ld, ptr(wc), stats.const_data_ptr<float>(), dt, wt == x.scalar_type() ? dt : ARCN_DTYPE_F32,
                                  out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), (float *)out_ptr(scratch), nf, r.n, (int)C, go.stream),
              "layer_norm_bwd");
-        return first_order(std::move(out), graph, "layer_norm");
+        return first_order(std::move(out), graph, "layer_norm", {x, w, g[0]});
     }
 };
 
@@ -269,7 +268,7 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
                 out[2] = db;
             }
         }
-        return first_order(std::move(out), graph, "linear_act_residual");
+        return first_order(std::move(out), graph, "linear_act_residual", {x, saved[1], b, g[0]});
     }
 };
 
@@ -343,7 +342,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
                 if (need(5)) out[5] = db.narrow(0, H, H);
             }
         }
-        return first_order(std::move(out), graph, "gated_ffn");
+        return first_order(std::move(out), graph, "gated_ffn", {x, saved[1], saved[2], saved[3], saved[4], saved[5], g[0]});
     }
 };
 

@@ -1,0 +1,66 @@
+"""Calls of layer norm, the dense layer and the gated block at the edges of what they take: second and forward-mode derivatives, traces, tails
+of the activations, the 256-wide kernels, sums that are exact, the calls without autograd."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def leaf(seed, *shape, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda().requires_grad_(True)
+
+
+# ---- second derivatives -----------------------------------------------------------------------------------------------------------------
+def small_calls():
+    """name -> (function of the leaves, leaves by name): all three operators with every operand a leaf"""
+    from arcnerf_amd.ops import autograd as A
+    x, r = leaf(1, 40, 16), leaf(2, 40, 16)
+    w, b, w2, wd = leaf(3, 16, 16), leaf(4, 16), leaf(5, 16, 16), leaf(6, 16, 16)
+    return {
+        'layer_norm': (lambda t: A.layer_norm(t['x'], t['w'], t['b']), dict(x=x, w=leaf(7, 16), b=b)),
+        'linear_act_residual': (lambda t: A.linear_act_residual(t['x'], t['w'], t['b'], t['r'], act='silu'), dict(x=x, w=w, b=b, r=r)),
+        'linear_act_residual without act': (lambda t: A.linear_act_residual(t['x'], t['w'], t['b'], t['r']), dict(x=x, w=w, b=b, r=r)),
+        'gated_ffn': (lambda t: A.gated_ffn(t['x'], t['wg'], t['wu'], t['wd'], t['bg'], t['bu'], t['bd'], t['r']),
+                      dict(x=x, wg=w, wu=w2, wd=wd, bg=b, bu=leaf(8, 16), bd=leaf(9, 16), r=r)),
+    }
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'linear_act_residual without act', 'gated_ffn'])
+def test_a_loss_on_gradients_raises_whatever_else_it_holds(name):
+    """a loss with a term in the result and one in its gradient: every way of differentiating it raises, none returns the first term alone"""
+    fn, t = small_calls()[name]
+    for wrt in t:
+        def loss():
+            y = fn(t)
+            g, = torch.autograd.grad(y.square().sum(), t[wrt], create_graph=True)
+            assert g.requires_grad
+            return y.sum() + g.square().sum()
+        for call in (lambda l: torch.autograd.grad(l, t['x']), lambda l: torch.autograd.grad(l, t['w' if 'w' in t else 'wd']), lambda l: l.backward(inputs=[t['x']]),
+                     lambda l: l.backward(), lambda l: torch.autograd.grad(l, t['x'], allow_unused=True)):
+            with pytest.raises(RuntimeError, match='differentiated once'):
+                call(loss())
+
+
+def test_a_loss_on_gradients_raises_through_the_incoming_gradient():
+    """only the incoming gradient depends on the leaf that is asked for"""
+    from arcnerf_amd.ops import autograd as A
+    x, w, s = leaf(1, 40, 16), leaf(2, 16, 16), leaf(3, 40, 16)
+    y = A.linear_act_residual(x.detach(), w, act='gelu')
+    g, = torch.autograd.grad((y * s).sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiated once'):
+        torch.autograd.grad(s.square().sum() + g.square().sum(), s)
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+def test_gradients_with_a_graph_are_the_gradients(name):
+    """create_graph alone changes no value, and other terms of a loss are differentiated as ever"""
+    fn, t = small_calls()[name]
+    leaves = list(t.values())
+    plain = torch.autograd.grad(fn(t).square().sum(), leaves)
+    graph = torch.autograd.grad(fn(t).square().sum(), leaves, create_graph=True)
+    for k, a, b in zip(t, plain, graph):
+        assert torch.equal(a, b), k
+    z = leaf(20, 5)
+    got, = torch.autograd.grad(z.square().sum() + graph[0].sum(), z)
+    assert torch.equal(got, 2 * z.detach())
