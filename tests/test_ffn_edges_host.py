@@ -1,0 +1,36 @@
+"""CPU checks of what the feed-forward layers' native nodes refuse before anything else, and of the modules on them."""
+import pytest
+import torch
+
+from arcnerf_amd import _native as N
+
+
+@pytest.fixture(scope='module')
+def nodes():
+    import os
+    if not os.path.exists(N.NODES_PATH):
+        import __graft_entry__ as ge
+        ge.build()
+    return N.torch_nodes()
+
+
+def node_calls(nodes):
+    """name -> (call of its operands, operands): every operand given"""
+    x, v, w = torch.randn(4, 8), torch.randn(8), torch.randn(8, 8)
+    return {
+        'layer_norm': (lambda x, w, b: nodes.layer_norm(x, w, b, 1e-5), [x, v, v]),
+        'linear_act_residual': (lambda x, w, b, r: nodes.linear_act_residual(x, w, b, r, 7, 1.0), [x, w, v, x]),
+        'gated_ffn': (lambda x, wg, wu, wd, bg, bu, bd, r: nodes.gated_ffn(x, wg, wu, wd, bg, bu, bd, r, 7, 1.0), [x, w, w, w, v, v, v, x]),
+    }
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+def test_a_tangent_in_any_operand_is_refused(nodes, name):
+    import torch.autograd.forward_ad as fw
+    call, ops = node_calls(nodes)[name]
+    with fw.dual_level():
+        for k in range(len(ops)):
+            for grad in (False, True):
+                with_dual = [fw.make_dual(t.detach().requires_grad_(grad), torch.ones_like(t)) if i == k else t for i, t in enumerate(ops)]
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    call(*with_dual)

@@ -64,3 +64,20 @@ def test_gradients_with_a_graph_are_the_gradients(name):
     z = leaf(20, 5)
     got, = torch.autograd.grad(z.square().sum() + graph[0].sum(), z)
     assert torch.equal(got, 2 * z.detach())
+
+
+# ---- forward-mode derivatives -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+def test_forward_mode_is_refused(name):
+    """a tangent in any operand, with and without a graph, and through torch.func: refused, never dropped"""
+    import torch.autograd.forward_ad as fw
+    fn, t = small_calls()[name]
+    with fw.dual_level():
+        for k in t:
+            for grad in (False, True):
+                dual = {j: fw.make_dual(v.detach().requires_grad_(grad), torch.ones_like(v)) if j == k else v.detach() for j, v in t.items()}
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    fn(dual)
+    x = t['x'].detach()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: fn(dict({j: u.detach() for j, u in t.items()}, x=v)), (x,), (torch.ones_like(x),))
