@@ -8,6 +8,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cstdlib>
@@ -123,8 +124,10 @@ bool needs_graph(std::initializer_list<const Tensor *> ts) {
     return false;
 }
 
-// a tangent would be dropped without a word: the kernels are launched on raw pointers
-void refuse_forward_mode(std::initializer_list<const Tensor *> ts, const char *what) {
+// The kernels are launched on raw pointers: a tangent would be dropped without a word, and a trace would record the allocation of a result and
+// nothing that fills it.
+void refuse_untracked(std::initializer_list<const Tensor *> ts, const char *what) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "arcnerf_amd: ", what, " cannot be traced (torch.jit.trace)");
     for (const Tensor *t : ts)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "arcnerf_amd: ", what, " has no forward-mode derivative");
 }
@@ -203,7 +206,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor &x, const OptTensor &w_, const OptTensor &b_, double eps) {
     const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
-    refuse_forward_mode({&x, &w, &b}, "layer_norm");
+    refuse_untracked({&x, &w, &b}, "layer_norm");
     return needs_graph({&x, &w, &b}) ? LayerNorm::apply(x, opt(w), opt(b), eps) : norm_forward(x, w, b, eps, nullptr);
 }
 
@@ -281,7 +284,7 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
 
 Tensor linear_act_residual(const Tensor &x, const Tensor &w, const OptTensor &b_, const OptTensor &res_, int64_t act, double beta) {
     const Tensor b = b_.value_or(Tensor()), res = res_.value_or(Tensor());
-    refuse_forward_mode({&x, &w, &b, &res}, "linear_act_residual");
+    refuse_untracked({&x, &w, &b, &res}, "linear_act_residual");
     return needs_graph({&x, &w, &b, &res}) ? LinearActResidual::apply(x, w, opt(b), opt(res), act, beta) : dense_forward(x, w, b, res, act, beta);
 }
 
@@ -357,7 +360,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 Tensor gated_ffn(const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &wd, const OptTensor &bg_, const OptTensor &bu_, const OptTensor &bd_,
                  const OptTensor &res_, int64_t act, double beta) {
     const Tensor bg = bg_.value_or(Tensor()), bu = bu_.value_or(Tensor()), bd = bd_.value_or(Tensor()), res = res_.value_or(Tensor());
-    refuse_forward_mode({&x, &wg, &wu, &wd, &bg, &bu, &bd, &res}, "gated_ffn");
+    refuse_untracked({&x, &wg, &wu, &wd, &bg, &bu, &bd, &res}, "gated_ffn");
     TORCH_CHECK(wd.dim() == 2 && wg.dim() == 2 && wd.size(1) == wg.size(0), "arcnerf_amd: w_down must be (N, H) for w_gate (H, K), got ", wd.sizes(), " and ", wg.sizes());
     if (needs_graph({&x, &wg, &wu, &wd, &bg, &bu, &bd, &res})) return GatedFfn::apply(x, wg, wu, wd, opt(bg), opt(bu), opt(bd), opt(res), act, beta);
     return dense_forward(gated_forward(x, wg, wu, bg, bu, act, beta), wd, bd, res, ARCN_ACT_NONE, 1.0);

@@ -34,3 +34,11 @@ def test_a_tangent_in_any_operand_is_refused(nodes, name):
                 with_dual = [fw.make_dual(t.detach().requires_grad_(grad), torch.ones_like(t)) if i == k else t for i, t in enumerate(ops)]
                 with pytest.raises(RuntimeError, match='forward-mode'):
                     call(*with_dual)
+
+
+@pytest.mark.filterwarnings('ignore::DeprecationWarning')
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+def test_a_trace_is_refused(nodes, name):
+    call, ops = node_calls(nodes)[name]
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        torch.jit.trace(call, tuple(ops))

@@ -81,3 +81,15 @@ def test_forward_mode_is_refused(name):
     x = t['x'].detach()
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda v: fn(dict({j: u.detach() for j, u in t.items()}, x=v)), (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.filterwarnings('ignore::DeprecationWarning')
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+def test_a_trace_is_refused(name):
+    """with and without a graph, also where only a captured parameter meets the traced input"""
+    fn, t = small_calls()[name]
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match='cannot be traced'):
+            torch.jit.trace(lambda x: fn(dict(t, x=x)), (t['x'].detach(),))
+    y = fn(t)                                   # (nothing of the failed trace stays)
+    assert torch.isfinite(y).all()
