@@ -95,7 +95,7 @@ __device__ __forceinline__ float act_eval(float z, float beta, float inv_beta, f
         if (SLOPE) slope = fmaf(z * 0.398942280f, e, cdf);
         return z * cdf;
     } else if constexpr (ACT == ARCN_ACT_GELU) {
-        const float cdf = 0.5f * (1.f + erff(z * 0.707106781f));
+        const float cdf = 0.5f * erfcf(z * -0.707106781f);      // (1 + erf cancels for negative z: nothing of it is left at -6)
         if (SLOPE) slope = fmaf(z * 0.398942280f, exp_hw(-0.5f * z * z), cdf);
         return z * cdf;
     } else {

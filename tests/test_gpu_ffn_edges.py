@@ -93,3 +93,44 @@ def test_a_trace_is_refused(name):
             torch.jit.trace(lambda x: fn(dict(t, x=x)), (t['x'].detach(),))
     y = fn(t)                                   # (nothing of the failed trace stays)
     assert torch.isfinite(y).all()
+
+
+# ---- tails of the activations -----------------------------------------------------------------------------------------------------------
+E24 = 2.0 ** -24
+
+
+def values_and_slopes(z, act, rows=None):
+    """act and act' at the numbers z, exactly the pre-activations of layers of one input with weight 1: of the dense layer's and the gated block's
+    kernels for few rows and for many"""
+    from arcnerf_amd.ops import autograd as A
+    one = torch.ones(1, 1, dtype=z.dtype, device='cuda')
+    for n in (z.numel(), 2000):
+        x = z.repeat(-(-n // z.numel()))[:, None].cuda().requires_grad_(True)
+        y = A.linear_act_residual(x, one, act=act)
+        s, = torch.autograd.grad(y.sum(), x)
+        yield 'dense', n, y[:z.numel(), 0].detach().double().cpu(), s[:z.numel(), 0].double().cpu()
+        # the up projection is 1 by its bias: h = act(z), dg = act'(z), dx = dg
+        y = A.gated_ffn(x, one, torch.zeros_like(one), one, b_up=one[0], act=act)
+        s, = torch.autograd.grad(y.sum(), x)
+        yield 'gated', n, y[:z.numel(), 0].detach().double().cpu(), s[:z.numel(), 0].double().cpu()
+
+
+def gelu64(z):
+    import math
+    cdf = 0.5 * torch.erfc(z * -math.sqrt(0.5))
+    phi = torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return z * cdf, cdf + z * phi
+
+
+def test_gelu_far_below_zero_f32():
+    """Relative to the value, e = 2^-24: the argument of erfc carries 2 e (a constant, a product), which its condition number, at most z^2 + 1,
+    carries on; erfcf 16 ulp = 32 e, the products 2 e.  The slope adds z phi: z^2 / 2 e of its exponent and 8 e of constants, products and the exponential,
+    and cancels against cdf, at most 0.21 of it from -2 on: 1 / (1 - 0.21) < 1.3."""
+    z = -torch.linspace(2, 9, 141)
+    y64, s64 = gelu64(z.double())
+    zz = z.double() ** 2
+    tol_y = (2 * (zz + 1) + 34) * E24
+    tol_s = 1.3 * (zz / 2 + 8 + 0.21 * tol_y / E24) * E24 + 2 * E24
+    for what, n, y, s in values_and_slopes(z, 'gelu'):
+        assert ((y - y64).abs() <= tol_y * y64.abs()).all(), (what, n)
+        assert ((s - s64).abs() <= tol_s * s64.abs()).all(), (what, n)
