@@ -46,9 +46,10 @@ __device__ __forceinline__ float exp_hw(float x) {
     return fmaf(e * 0.693147181f, lo, e);
 }
 
-// FAST (16-bit results): the exponential without that correction (x 2^-24 of itself, 2^-18 at most where the result counts) and the error
-// function by Abramowitz and Stegun 7.1.26 (1.5e-7), which shares its exponential with the slope: a third of the instructions of an epilogue
-// that is all of a wide tile's vector work
+// FAST (16-bit results): the exponential without that correction (x 2^-24 of itself, 2^-18 at most where the result counts) and
+// erfc(x) = t P(t) e^(-x^2), t = 1 / (1 + 0.38 x), which shares its exponential with the slope: a third of the instructions of an epilogue that
+// is all of a wide tile's vector work.  P: our own fit of degree 6, by the largest error relative to erfc in its tail (1.5e-5, 2^-5 of half a
+// step of f16, where a form with a small absolute error loses steps) and absolute towards zero (2.5e-7).
 template <int ACT, bool SLOPE, bool FAST>
 __device__ __forceinline__ float act_eval(float z, float beta, float inv_beta, float &slope) {
     if constexpr (ACT == ARCN_ACT_RELU) {
@@ -85,12 +86,14 @@ __device__ __forceinline__ float act_eval(float z, float beta, float inv_beta, f
         const float l = u == 1.f ? t : __logf(u) * (t * __builtin_amdgcn_rcpf(u - 1.f));
         return bz > 20.f ? z : (fmaxf(bz, 0.f) + l) * inv_beta;
     } else if constexpr (FAST && ACT == ARCN_ACT_GELU) {
-        const float e = __builtin_amdgcn_exp2f(z * z * -0.721347520f);                                   // e^(-z^2 / 2)
-        const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.231641888f, 1.f));                        // 1 / (1 + p |z| / sqrt 2)
-        float q = fmaf(t, 1.061405429f, -1.453152027f);
-        q = fmaf(t, q, 1.421413741f);
-        q = fmaf(t, q, -0.284496736f);
-        q = fmaf(t, q, 0.254829592f) * t * e * 0.5f;                                                     // half of erfc(|z| / sqrt 2)
+        const float e = __builtin_amdgcn_exp2f(z * z * -0.721347520f);             // e^(-z^2 / 2)
+        const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.26870057f, 1.f));   // 1 / (1 + 0.38 |z| / sqrt 2)
+        float q = fmaf(t, -0.0584391914f, 0.152983919f);
+        q = fmaf(t, q, -0.0142182391f);
+        q = fmaf(t, q, 0.109800145f);
+        q = fmaf(t, q, 0.0951927528f);
+        q = fmaf(t, q, 0.107490107f);
+        q = fmaf(t, q, 0.107190385f) * t * e;                                      // half of erfc(|z| / sqrt 2)
         const float cdf = z > 0.f ? 1.f - q : q;
         if (SLOPE) slope = fmaf(z * 0.398942280f, e, cdf);
         return z * cdf;

@@ -134,3 +134,15 @@ def test_gelu_far_below_zero_f32():
     for what, n, y, s in values_and_slopes(z, 'gelu'):
         assert ((y - y64).abs() <= tol_y * y64.abs()).all(), (what, n)
         assert ((s - s64).abs() <= tol_s * s64.abs()).all(), (what, n)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=['bf16', 'f16'])
+def test_gelu_far_below_zero_16_bits(dtype):
+    """every number of the type in [-9, -2]: half a step of the result's type, and 2e-5 of the evaluation (the fit 1.5e-5, the exponent's rounding
+    z^2 / 2 2^-24 and those of the products)"""
+    z = -torch.arange(2.0, 9.0, 2.0 ** -9).to(dtype).unique()
+    half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    y64, s64 = gelu64(z.double())
+    for what, n, y, s in values_and_slopes(z, 'gelu'):
+        assert ((y - y64).abs() <= (half + 2e-5) * y64.abs() + least).all(), (what, n)
+        assert ((s - s64).abs() <= (half + 2e-5) * s64.abs() + least).all(), (what, n)
