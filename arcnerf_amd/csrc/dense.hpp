@@ -55,17 +55,15 @@ __device__ __forceinline__ float act_eval(float z, float beta, float inv_beta, f
     if constexpr (ACT == ARCN_ACT_RELU) {
         if (SLOPE) slope = z <= 0.f ? 0.f : 1.f;
         return z <= 0.f ? 0.f : z;      // (a NaN stays one)
-    } else if constexpr (FAST && (ACT == ARCN_ACT_SIGMOID || ACT == ARCN_ACT_SILU)) {
+    } else if constexpr (FAST && ACT == ARCN_ACT_SIGMOID && !SLOPE) {
+        return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+    } else if constexpr (FAST && ACT == ARCN_ACT_SILU) {
         const float q = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
-        if constexpr (ACT == ARCN_ACT_SIGMOID) {
-            if (SLOPE) slope = q * (1.f - q);
-            return q;
-        } else {
-            if (SLOPE) slope = q * fmaf(z, 1.f - q, 1.f);
-            return z * q;
-        }
+        if (SLOPE) slope = q * fmaf(z, 1.f - q, 1.f);
+        return z * q;
     } else if constexpr (ACT == ARCN_ACT_SIGMOID || ACT == ARCN_ACT_SILU) {
-        const float e = exp_hw(-fabsf(z)), q = __builtin_amdgcn_rcpf(1.f + e), eq = e * q;
+        // (the slope as e q^2: q (1 - q) cancels from z of about 8 on, its digits are gone at 17)
+        const float e = FAST ? __builtin_amdgcn_exp2f(fabsf(z) * -1.44269504f) : exp_hw(-fabsf(z)), q = __builtin_amdgcn_rcpf(1.f + e), eq = e * q;
         const bool up = z >= 0.f;
         const float s = up ? q : eq;
         if constexpr (ACT == ARCN_ACT_SIGMOID) {

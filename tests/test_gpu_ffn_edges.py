@@ -146,3 +146,16 @@ def test_gelu_far_below_zero_16_bits(dtype):
     for what, n, y, s in values_and_slopes(z, 'gelu'):
         assert ((y - y64).abs() <= (half + 2e-5) * y64.abs() + least).all(), (what, n)
         assert ((s - s64).abs() <= (half + 2e-5) * s64.abs() + least).all(), (what, n)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+def test_sigmoid_slope_far_from_zero(dtype):
+    """s (1 - s) relative to its value on both sides of zero, e = 2^-24: the exponent's rounding |z| e (16 bits; f32 puts it back), 16 e of the
+    exponential, the reciprocal and the products, and half a step of the result"""
+    z = torch.cat([torch.arange(4.0, 30.0, 2.0 ** -4), -torch.arange(4.0, 30.0, 2.0 ** -4)]).to(dtype)
+    half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    zz = z.double()
+    y64, s64 = torch.sigmoid(zz), torch.sigmoid(zz) * torch.sigmoid(-zz)
+    for what, n, y, s in values_and_slopes(z, 'sigmoid'):
+        assert ((y - y64).abs() <= (half + (zz.abs() + 16) * E24) * y64 + least).all(), (what, n)
+        assert ((s - s64).abs() <= (half + 1.01 * (zz.abs() + 16) * E24) * s64 + least).all(), (what, n)
