@@ -33,6 +33,8 @@ class GeoNet(EncoderMLPGeoNet):
         if block_cfg is not None:
             # hidden layers 1 .. D - 1 as residual blocks (base_modules/ffn.py): the residual takes the place of the skip concatenation
             assert len(self.skips) == 0 and not use_siren and not weight_norm, 'residual blocks take no skips, siren or weight norm'
+            # (the first and last layer alone make no sphere: blocks add their own random parts to what passes between them)
+            assert not geometric_init or D == 1, 'residual blocks take no part in the geometric initialisation: set geometric_init to False'
         layers = []
         for i in range(D + 1):
             after_skip = i > 0 and (i - 1) in self.skips

@@ -42,3 +42,26 @@ def test_a_trace_is_refused(nodes, name):
     call, ops = node_calls(nodes)[name]
     with pytest.raises(RuntimeError, match='cannot be traced'):
         torch.jit.trace(call, tuple(ops))
+
+
+# ---- the modules --------------------------------------------------------------------------------------------------------------------------
+FREQ = {'type': 'FreqEmbedder', 'input_dim': 3, 'n_freqs': 0}      # the coordinates themselves (the encoding kernel runs on the GPU only)
+
+
+@pytest.mark.parametrize('block', [{'type': 'dense'}, {'type': 'gated'}], ids=['dense', 'gated'])
+def test_blocks_refuse_the_geometric_initialisation(block):
+    """which is on by default and makes a sphere of plain layers only"""
+    from arcnerf_amd.models.base_modules import build_geo_model
+    from arcnerf_amd.utils.cfgs_utils import dict_to_obj
+    cfg = {'W': 32, 'D': 4, 'skips': [], 'W_feat': 0, 'encoder': FREQ, 'block_cfg': block}
+    for more in ({}, {'geometric_init': True}):
+        with pytest.raises(AssertionError, match='geometric'):
+            build_geo_model(dict_to_obj(dict(cfg, **more)))
+    net = build_geo_model(dict_to_obj(dict(cfg, geometric_init=False)))
+    assert len(net.layers) == 5
+    # without blocks, and with no layer that would be one, the initialisation is there as ever
+    torch.manual_seed(0)
+    x = torch.nn.functional.normalize(torch.randn(500, 3), dim=-1) * 2
+    for more in ({'block_cfg': None}, {'D': 1}):
+        sdf, _ = build_geo_model(dict_to_obj(dict(cfg, W=256, geometric_init=True, **more)))(x)
+        assert (sdf - 1).abs().mean().item() < 0.5
