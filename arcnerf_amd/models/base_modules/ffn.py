@@ -17,6 +17,14 @@ def _as(t, dtype):
     return t if t is None else t.to(dtype)
 
 
+def _add_to_stream(x, h, branch):
+    """x + branch(residual) in x's type: in the branch's last epilogue where h, x in the type that the branch computes in, holds all of x; else
+    outside, so that neither the stream nor its gradient loses bits to a narrower branch"""
+    if torch.promote_types(x.dtype, h.dtype) == h.dtype:
+        return branch(h).to(x.dtype)
+    return (x + branch(None)).to(x.dtype)
+
+
 class LayerNorm(nn.Module):
     """torch.nn.LayerNorm over the last dimension (same parameters and state_dict keys)"""
 
@@ -32,7 +40,7 @@ class LayerNorm(nn.Module):
 
 class ResidualDenseLayer(Linear):
     """x + act(norm(x) W^T + b): one norm and one product whose epilogue adds the bias, the activation and the residual.  `dtype` is the type the
-    layer computes in (its parameters stay float32)"""
+    layer computes in (its parameters stay float32, and a wider x keeps its type and bits: _add_to_stream)"""
 
     def __init__(self, dim, act='relu', beta=1.0, norm=True, bias=True, dtype=torch.float32):
         super().__init__(dim, dim, bias=bias)
@@ -43,11 +51,13 @@ class ResidualDenseLayer(Linear):
         from ...ops.autograd import linear_act_residual
         h = x.to(self.dtype)
         n = h if self.norm is None else self.norm(h)
-        return linear_act_residual(n, _as(self.weight, self.dtype), _as(self.bias, self.dtype), h, act=self.act, beta=self.beta).to(x.dtype)
+        w, b = _as(self.weight, self.dtype), _as(self.bias, self.dtype)
+        return _add_to_stream(x, h, lambda res: linear_act_residual(n, w, b, res, act=self.act, beta=self.beta))
 
 
 class GatedFfnBlock(nn.Module):
-    """x + down(act(gate(n)) * up(n)), n = norm(x): `gate` and `up` as one kernel, the residual in the epilogue of `down`"""
+    """x + down(act(gate(n)) * up(n)), n = norm(x): `gate` and `up` as one kernel, the residual in the epilogue of `down`.  `dtype` as
+    ResidualDenseLayer has it"""
 
     def __init__(self, dim, hidden, act='silu', beta=1.0, norm=True, bias=True, dtype=torch.float32):
         super().__init__()
@@ -61,8 +71,9 @@ class GatedFfnBlock(nn.Module):
         d = self.dtype
         h = x.to(d)
         n = h if self.norm is None else self.norm(h)
-        return gated_ffn(n, _as(self.gate.weight, d), _as(self.up.weight, d), _as(self.down.weight, d), _as(self.gate.bias, d), _as(self.up.bias, d),
-                         _as(self.down.bias, d), residual=h, act=self.act, beta=self.beta).to(x.dtype)
+        w = [_as(layer.weight, d) for layer in (self.gate, self.up, self.down)]
+        b = [_as(layer.bias, d) for layer in (self.gate, self.up, self.down)]
+        return _add_to_stream(x, h, lambda res: gated_ffn(n, *w, *b, residual=res, act=self.act, beta=self.beta))
 
 
 def build_block(cfg, dim, bias=True):

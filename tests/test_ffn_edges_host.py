@@ -65,3 +65,30 @@ def test_blocks_refuse_the_geometric_initialisation(block):
     for more in ({'block_cfg': None}, {'D': 1}):
         sdf, _ = build_geo_model(dict_to_obj(dict(cfg, W=256, geometric_init=True, **more)))(x)
         assert (sdf - 1).abs().mean().item() < 0.5
+
+
+STREAMS = [(torch.float32, 'bfloat16'), (torch.float32, 'float16'), (torch.float16, 'bfloat16'), (torch.bfloat16, 'float32'), (torch.float32, 'float32')]
+
+
+def check_stream(x_type, dtype, kind, device):
+    """a block whose branch is zero hands x and its gradient on, bit for bit"""
+    from arcnerf_amd.models.base_modules import build_block
+    from arcnerf_amd.utils.cfgs_utils import dict_to_obj
+    block = build_block(dict_to_obj({'type': kind, 'dtype': dtype, 'act': 'silu'}), 24).to(device)
+    last = block.down if kind == 'gated' else block
+    torch.nn.init.zeros_(last.weight)
+    torch.nn.init.zeros_(last.bias)
+    g = torch.Generator().manual_seed(0)
+    x = (torch.randn(30, 24, generator=g) * 3 + 0.123).to(x_type).to(device).requires_grad_(True)
+    y = block(x)
+    assert y.dtype == x_type and torch.equal(y, x)
+    dy = torch.randn(30, 24, generator=g).to(x_type).to(device)
+    dx, dw = torch.autograd.grad(y, [x, last.weight], dy)
+    assert torch.equal(dx, dy)              # (a zero weight hands no gradient to the branch's input)
+    assert dw.dtype == torch.float32 and torch.isfinite(dw).all()
+
+
+@pytest.mark.parametrize('kind', ['gated', 'dense'])
+@pytest.mark.parametrize('x_type,dtype', STREAMS)
+def test_a_narrow_branch_leaves_a_wide_stream_its_bits(x_type, dtype, kind):
+    check_stream(x_type, dtype, kind, 'cpu')

@@ -159,3 +159,11 @@ def test_sigmoid_slope_far_from_zero(dtype):
     for what, n, y, s in values_and_slopes(z, 'sigmoid'):
         assert ((y - y64).abs() <= (half + (zz.abs() + 16) * E24) * y64 + least).all(), (what, n)
         assert ((s - s64).abs() <= (half + 1.01 * (zz.abs() + 16) * E24) * s64 + least).all(), (what, n)
+
+
+# ---- the modules ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('kind', ['gated', 'dense'])
+def test_a_narrow_branch_leaves_a_wide_stream_its_bits(kind):
+    from test_ffn_edges_host import STREAMS, check_stream
+    for x_type, dtype in STREAMS:
+        check_stream(x_type, dtype, kind, 'cuda')
