@@ -9,6 +9,8 @@ static bool dense_act(int act, float beta) {
     return act == ARCN_ACT_NONE || act == ARCN_ACT_RELU || act == ARCN_ACT_SIGMOID || act == ARCN_ACT_SILU || act == ARCN_ACT_GELU;
 }
 static bool dense_sizes(int64_t rows, int a, int b) { return rows >= 0 && a >= 1 && b >= 1 && a <= (1 << 24) && b <= (1 << 24); }
+// of the backward's products: N may be the two halves of a gated layer side by side
+static bool dense_sizes_n(int64_t rows, int K, int N) { return N >= 1 && dense_sizes(rows, K, N - N / 2); }
 
 }  // namespace arcn
 
@@ -35,20 +37,20 @@ ARCN_EXPORT int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const 
 }
 
 ARCN_EXPORT int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int dtype, int64_t n_rows, int N, int K, void *stream) {
-    if (!dense_type(dtype) || !dense_sizes(n_rows, K, N) || (w2 && (N & 1))) return einval("dense_dx: unsupported type or size");
+    if (!dense_type(dtype) || !dense_sizes_n(n_rows, K, N) || (w2 && (N & 1))) return einval("dense_dx: unsupported type or size");
     if (n_rows == 0) return ARCN_OK;
     if (!dz || !w || !dx || ld_dz < N) return einval("dense_dx: missing / invalid argument");
     return ARCN_DENSE_DISPATCH(dx(dz, ld_dz, w, w2, dx, n_rows, N, K, as_stream(stream)));
 }
 
 ARCN_EXPORT int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K, int dtype) {
-    if (!dense_sizes(n_rows, K, N) || !dense_type(dtype)) return 0;
+    if (!dense_sizes_n(n_rows, K, N) || !dense_type(dtype)) return 0;
     return (int64_t)dense_dw_slabs(dtype == ARCN_DTYPE_F32 ? 4 : 2, n_rows, N, K) * ((int64_t)N * K + N);
 }
 
 ARCN_EXPORT int arcn_dense_dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, int dtype, float *scratch, int64_t scratch_floats,
                               int64_t n_rows, int N, int K, void *stream) {
-    if (!dense_type(dtype) || !dense_sizes(n_rows, K, N)) return einval("dense_dw: unsupported type or size");
+    if (!dense_type(dtype) || !dense_sizes_n(n_rows, K, N)) return einval("dense_dw: unsupported type or size");
     if (!dw || !scratch || (n_rows > 0 && (!dz || !x || ld_dz < N || ld_x < K))) return einval("dense_dw: missing / invalid argument");
     if (scratch_floats < arcn_dense_dw_scratch_floats(n_rows, N, K, dtype)) return einval("dense_dw: scratch smaller than arcn_dense_dw_scratch_floats");
     return ARCN_DENSE_DISPATCH(dw(dz, ld_dz, x, ld_x, dw, db, scratch, n_rows, N, K, as_stream(stream)));

@@ -92,3 +92,20 @@ def check_stream(x_type, dtype, kind, device):
 @pytest.mark.parametrize('x_type,dtype', STREAMS)
 def test_a_narrow_branch_leaves_a_wide_stream_its_bits(x_type, dtype, kind):
     check_stream(x_type, dtype, kind, 'cpu')
+
+
+# ---- sizes ------------------------------------------------------------------------------------------------------------------------------
+def test_backward_products_take_what_a_gated_forward_takes(nodes):
+    """a hidden width of up to 2^24 is two halves of that in the backward (no rows: nothing is launched)"""
+    lib, n = N.lib(), None
+    for hid in (1 << 23, (1 << 23) + 1, 1 << 24):
+        assert lib.arcn_gated_fwd(n, 1, n, n, n, n, n, 0, 7, 1.0, 0, 1, hid, n) == 0
+        assert lib.arcn_gated_bwd(n, 1, n, n, n, n, n, 1, n, n, 0, 7, 1.0, 0, 1, hid, 1, n) == 0
+        assert lib.arcn_dense_dx(n, 2 * hid, n, n, n, 0, 0, 2 * hid, 1, n) == 0
+        assert lib.arcn_dense_dw_scratch_floats(1, 2 * hid, 1, 0) >= 4 * hid
+    for big in ((1 << 25) + 1, (1 << 31) - 1):
+        assert lib.arcn_dense_dx(n, big, n, n, n, 0, 0, big, 1, n) == -1
+        assert lib.arcn_dense_dw_scratch_floats(1, big, 1, 0) == 0
+    for bad in (0, -1, -(1 << 31)):
+        assert lib.arcn_dense_dx(n, 1, n, n, n, 0, 0, bad, 1, n) == -1
+        assert lib.arcn_dense_dw_scratch_floats(1, bad, 1, 0) == 0

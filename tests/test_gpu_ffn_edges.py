@@ -167,3 +167,18 @@ def test_a_narrow_branch_leaves_a_wide_stream_its_bits(kind):
     from test_ffn_edges_host import STREAMS, check_stream
     for x_type, dtype in STREAMS:
         check_stream(x_type, dtype, kind, 'cuda')
+
+
+# ---- sizes and sums that are exact ------------------------------------------------------------------------------------------------------
+def test_gated_widest_hidden_layer():
+    """more than 2^23 hidden features, whose two halves are more than 2^24 in the backward; everything in {-1, 0, 1}, so every sum is exact"""
+    from arcnerf_amd.ops import autograd as A
+    hid = (1 << 23) + 72
+    g = torch.Generator(device='cuda').manual_seed(0)
+    wg, wu, wd = (torch.randint(-1, 2, (hid,), generator=g, device='cuda').float() for _ in range(3))
+    x = torch.ones(1, 1, device='cuda', requires_grad=True)
+    leaves = [x] + [w.clone().requires_grad_(True) for w in (wg[:, None], wu[:, None], wd[None])]
+    y = A.gated_ffn(*leaves, act=None)
+    dx, dwg, dwu, dwd = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    assert y.item() == (wg * wu * wd).double().sum().item() and dx.item() == 2 * (wg * wu * wd).double().sum().item()
+    assert torch.equal(dwg[:, 0], wd * wu) and torch.equal(dwu[:, 0], wd * wg) and torch.equal(dwd[0], wg * wu)
