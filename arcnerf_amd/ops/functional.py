@@ -1266,6 +1266,7 @@ def layer_norm_bwd(x, dy, weight, stats, want_dx=True, want_dw=True, want_db=Tru
     wt = weight.dtype if weight is not None else (param_dtype or x.dtype)
     if tuple(stats.shape) != (S, 2) or stats.dtype != torch.float32 or stats.device != x.device:
         raise RuntimeError('arcnerf_amd: stats must be the ({}, 2) float32 that layer_norm_fwd gave'.format(S))
+    stats = stats.contiguous()
     dx = _fresh((S, C), x.dtype, x.device) if want_dx else None
     if S == 0:
         return dx, *(torch.zeros(C, dtype=wt, device=x.device) if want else None for want in (want_dw, want_db))
@@ -1274,7 +1275,7 @@ def layer_norm_bwd(x, dy, weight, stats, want_dx=True, want_dw=True, want_db=Tru
     nf = int(N.lib().arcn_layer_norm_bwd_scratch_floats(S, C, _DTYPE[x.dtype])) if want_dw or want_db else 0
     scratch = torch.empty(nf, dtype=torch.float32, device=x.device) if nf else None
     with _device_of(x):
-        N.check(N.lib().arcn_layer_norm_bwd(x.data_ptr(), ld, dy.data_ptr(), ld_dy, N.ptr(weight), N.ptr(stats.contiguous()), _DTYPE[x.dtype], _DTYPE[wt],
+        N.check(N.lib().arcn_layer_norm_bwd(x.data_ptr(), ld, dy.data_ptr(), ld_dy, N.ptr(weight), N.ptr(stats), _DTYPE[x.dtype], _DTYPE[wt],
                                             N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(scratch), nf, S, C, N.stream()), 'layer_norm_bwd')
     return dx, dw, db
 

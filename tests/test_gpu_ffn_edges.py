@@ -182,3 +182,95 @@ def test_gated_widest_hidden_layer():
     dx, dwg, dwu, dwd = torch.autograd.grad(y, leaves, torch.ones_like(y))
     assert y.item() == (wg * wu * wd).double().sum().item() and dx.item() == 2 * (wg * wu * wd).double().sum().item()
     assert torch.equal(dwg[:, 0], wd * wu) and torch.equal(dwu[:, 0], wd * wg) and torch.equal(dwd[0], wg * wu)
+
+
+# ---- the calls without autograd ---------------------------------------------------------------------------------------------------------
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ['f32', 'bf16', 'f16']
+
+
+def wide_rows(seed, rows, width, dtype):
+    """a column slice of a wider buffer"""
+    return leaf(seed, rows, width + 5, dtype=dtype).detach()[:, 3:3 + width]
+
+
+def same(a, b):
+    assert len(a) == len(b)
+    for k, (u, v) in enumerate(zip(a, b)):
+        assert (u is None) == (v is None) and (u is None or (u.dtype == v.dtype and torch.equal(u, v))), k
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,width', [(1, 8), (37, 45), (300, 256), (0, 16)])
+def test_layer_norm_calls_are_the_nodes(dtype, rows, width):
+    from arcnerf_amd.ops import autograd as A, functional as F
+    for wt in (dtype, torch.float32):
+        x, dy = wide_rows(1, rows, width, dtype), wide_rows(2, rows, width, dtype)
+        w, b = leaf(3, width, dtype=wt), leaf(4, width, dtype=wt)
+        xg = x.detach().requires_grad_(True)
+        y, stats = F.layer_norm_fwd(x, w.detach(), b.detach(), want_stats=True)
+        yn = A.layer_norm(xg, w, b)
+        same((y, F.layer_norm_fwd(x, w.detach(), b.detach())), (yn.detach(),) * 2)
+        want = torch.autograd.grad(yn, [xg, w, b], dy)
+        same(F.layer_norm_bwd(x, dy, w.detach(), stats), want)
+        spread = torch.full((rows, 5), float('nan'), device='cuda')
+        spread[:, 1:3] = stats                                              # statistics that are not contiguous
+        same(F.layer_norm_bwd(x, dy, w.detach(), spread[:, 1:3], want_dx=False), (None,) + want[1:])
+        same(F.layer_norm_bwd(x, dy, w.detach(), stats, want_dw=False, want_db=False), (want[0], None, None))
+        # no weight: the type of the bias's gradient is the caller's
+        bn = leaf(4, width, dtype=wt)
+        db, = torch.autograd.grad(A.layer_norm(x, None, bn), bn, dy)
+        same(F.layer_norm_bwd(x, dy, None, stats, want_dx=False, want_dw=False, param_dtype=wt), (None, None, db))
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,n', [(1, 8, 8), (37, 45, 21), (500, 128, 72), (17000, 40, 56), (0, 16, 8)])
+def test_dense_calls_are_the_nodes(dtype, rows, k, n):
+    from arcnerf_amd.ops import autograd as A, functional as F
+    x, dy, r = wide_rows(1, rows, k, dtype), wide_rows(2, rows, n, dtype), wide_rows(3, rows, n, dtype)
+    w, b = leaf(4, n, k, dtype=dtype, scale=0.2), leaf(5, n, dtype=dtype)
+    wd, bd = w.detach(), b.detach()
+    for act in ('gelu', 'softplus', None):
+        xg = x.detach().requires_grad_(True)
+        y = A.linear_act_residual(xg, w, b, r, act=act, beta=2.0)
+        same((F.dense_fwd(x, wd, bd, r, act, 2.0),), (y.detach(),))
+        want = torch.autograd.grad(y, [xg, w, b], dy)
+        dz, dx = F.dense_dz(x, wd, bd, dy, act, 2.0, want_dx=True)
+        same((dx,) + F.dense_dw(dz, x, want_db=True), want)
+        same(F.dense_dw(dz, x), (want[1], None))
+        if act is None or rows < 16384:                                     # (else dx comes from the kernel of dz, in another order of sums)
+            alone = F.dense_dz(x, wd, bd, dy, act, 2.0)
+            same((alone, F.dense_dx(alone, wd)), (dz, dx))
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,hid,n', [(1, 8, 16, 8), (37, 45, 21, 30), (700, 64, 136, 72), (0, 8, 8, 8)])
+def test_gated_calls_are_the_nodes(dtype, rows, k, hid, n):
+    from arcnerf_amd.ops import autograd as A, functional as F
+    x, dy, r = wide_rows(1, rows, k, dtype), wide_rows(2, rows, n, dtype), wide_rows(3, rows, n, dtype)
+    p = {'wg': leaf(4, hid, k, dtype=dtype, scale=0.2), 'wu': leaf(5, hid, k, dtype=dtype, scale=0.2), 'wd': leaf(6, n, hid, dtype=dtype, scale=0.2),
+         'bg': leaf(7, hid, dtype=dtype), 'bu': leaf(8, hid, dtype=dtype), 'bd': leaf(9, n, dtype=dtype)}
+    q = {name: t.detach() for name, t in p.items()}
+    xg = x.detach().requires_grad_(True)
+    y = A.gated_ffn(xg, p['wg'], p['wu'], p['wd'], p['bg'], p['bu'], p['bd'], r, act='silu')
+    h = F.gated_fwd(x, q['wg'], q['wu'], q['bg'], q['bu'])
+    same((F.dense_fwd(h, q['wd'], q['bd'], r),), (y.detach(),))
+    want = dict(zip(['x'] + list(p), torch.autograd.grad(y, [xg] + list(p.values()), dy)))
+    dgu = F.gated_bwd(x, q['wg'], q['wu'], q['bg'], q['bu'], dy, q['wd'])
+    dw, db = F.dense_dw(dgu, x, want_db=True)
+    same((F.dense_dx(dgu, q['wg'], q['wu']), dw[:hid], dw[hid:], db[:hid], db[hid:]) + F.dense_dw(dy, h, want_db=True),
+         tuple(want[name] for name in ('x', 'wg', 'wu', 'bg', 'bu', 'wd', 'bd')))
+
+
+def test_calls_without_autograd_refuse():
+    from arcnerf_amd.ops import functional as F
+    x, w, st = torch.zeros(4, 8, device='cuda'), torch.zeros(6, 8, device='cuda'), torch.zeros(4, 2, device='cuda')
+    bad = [lambda: F.layer_norm_bwd(x, x, None, st[:3]), lambda: F.layer_norm_bwd(x, x, None, st.half()), lambda: F.layer_norm_bwd(x, x[:3], None, st),
+           lambda: F.layer_norm_bwd(x, x, torch.ones(7, device='cuda'), st), lambda: F.dense_dz(x, w, None, x, 'silu'), lambda: F.dense_dz(x, w, None, x[:, :6].half(), 'silu'),
+           lambda: F.dense_dx(x, w), lambda: F.dense_dx(x[:, :7], w[:3], w[:3]), lambda: F.dense_dx(x, w[:4], w[:3]), lambda: F.dense_dw(x, x[:3]),
+           lambda: F.gated_fwd(x, w, w[:5]), lambda: F.gated_bwd(x, w, w, None, None, x, torch.zeros(8, 5, device='cuda')),
+           lambda: F.gated_bwd(x, w, w, None, None, x[:, :7], torch.zeros(8, 6, device='cuda'))]
+    for k, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail('call {} went through'.format(k))
