@@ -1264,6 +1264,8 @@ def layer_norm_bwd(x, dy, weight, stats, want_dx=True, want_dw=True, want_db=Tru
     dy, ld_dy = _ffn_rows('dy', dy, C, like=x)
     weight = _ffn_param('weight', weight, (C,), x, (x.dtype, torch.float32))
     wt = weight.dtype if weight is not None else (param_dtype or x.dtype)
+    if wt not in (x.dtype, torch.float32):
+        raise RuntimeError('arcnerf_amd: the parameters of {} rows are {} or float32, not {}'.format(x.dtype, x.dtype, wt))
     if tuple(stats.shape) != (S, 2) or stats.dtype != torch.float32 or stats.device != x.device:
         raise RuntimeError('arcnerf_amd: stats must be the ({}, 2) float32 that layer_norm_fwd gave'.format(S))
     stats = stats.contiguous()

@@ -265,7 +265,8 @@ def test_gated_calls_are_the_nodes(dtype, rows, k, hid, n):
 def test_calls_without_autograd_refuse():
     from arcnerf_amd.ops import functional as F
     x, w, st = torch.zeros(4, 8, device='cuda'), torch.zeros(6, 8, device='cuda'), torch.zeros(4, 2, device='cuda')
-    bad = [lambda: F.layer_norm_bwd(x, x, None, st[:3]), lambda: F.layer_norm_bwd(x, x, None, st.half()), lambda: F.layer_norm_bwd(x, x[:3], None, st),
+    bad = [lambda: F.layer_norm_bwd(x, x, None, st, param_dtype=torch.float64), lambda: F.layer_norm_bwd(x, x, None, st, param_dtype=torch.bfloat16),
+           lambda: F.layer_norm_bwd(x, x, None, st[:3]), lambda: F.layer_norm_bwd(x, x, None, st.half()), lambda: F.layer_norm_bwd(x, x[:3], None, st),
            lambda: F.layer_norm_bwd(x, x, torch.ones(7, device='cuda'), st), lambda: F.dense_dz(x, w, None, x, 'silu'), lambda: F.dense_dz(x, w, None, x[:, :6].half(), 'silu'),
            lambda: F.dense_dx(x, w), lambda: F.dense_dx(x[:, :7], w[:3], w[:3]), lambda: F.dense_dx(x, w[:4], w[:3]), lambda: F.dense_dw(x, x[:3]),
            lambda: F.gated_fwd(x, w, w[:5]), lambda: F.gated_bwd(x, w, w, None, None, x, torch.zeros(8, 5, device='cuda')),
