@@ -275,3 +275,129 @@ def test_calls_without_autograd_refuse():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail('call {} went through'.format(k))
+
+
+# ---- exact sums: a row, a tile or a slab that is lost or counted twice changes them, whatever the number of rows --------------------------
+def ints(seed, *shape, dtype):
+    """-1, 0, 1: products and sums of up to 2^24 of them are exact in float32"""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    return torch.randint(-1, 2, shape, generator=g, device='cuda').to(dtype)
+
+
+def exact(a, b):
+    """a product of integers, float64"""
+    return a.double() @ b.double()
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,n', [(1, 1, 1), (255, 24, 40), (1000, 7, 3), (33001, 129, 130), (16400, 128, 72), (70001, 63, 31), (17000, 256, 256), (20003, 520, 520),
+                                      (33100, 520, 520), (66000, 264, 264), (300007, 16, 16)])
+def test_dense_sums_are_exact(dtype, rows, k, n):
+    """forward, dx, dW and db of the layer without an activation and of one whose activation is the identity (relu above zero: the kernels that compute
+    the slope): integers, rounded once.  At most 300007 terms, 2^18.2; a bias of 1024 is above any sum of 520 terms."""
+    from arcnerf_amd.ops import autograd as A
+    x, w, r, dy = ints(1, rows, k, dtype=dtype), ints(2, n, k, dtype=dtype), ints(3, rows, n, dtype=dtype), ints(4, rows, n, dtype=dtype)
+    z, dx, dw, db = exact(x, w.t()), exact(dy, w), exact(dy.t(), x), dy.double().sum(0)
+    for act, offset in ((None, 1), ('relu', 1024)):
+        b = torch.full((n,), offset, dtype=dtype, device='cuda')
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = A.linear_act_residual(*leaves, r, act=act)
+        assert torch.equal(y.detach(), (z + offset + r.double()).to(dtype)), (act, 'y')
+        for name, got, want in zip(('dx', 'dw', 'db'), torch.autograd.grad(y, leaves, dy), (dx, dw, db)):
+            assert torch.equal(got, want.to(dtype)), (act, name)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,hid,n', [(1, 1, 1, 1), (300, 24, 40, 16), (8301, 130, 260, 136), (33000, 264, 520, 264), (50001, 256, 264, 256)])
+def test_gated_sums_are_exact(dtype, rows, k, hid, n):
+    """the block without an activation, all of it integers: h = g u, du = dh g and dg = dh u are rounded to the type, every result once.  Sums of
+    k <= 264 terms are below 2^9, h below 2^18, dh below 2^9 (n <= 264) and the others far inside 2^24 (random signs: 2^8.5 sqrt(33000))."""
+    from arcnerf_amd.ops import autograd as A
+    x, dy, r = ints(1, rows, k, dtype=dtype), ints(2, rows, n, dtype=dtype), ints(3, rows, n, dtype=dtype)
+    wg, wu, wd = ints(4, hid, k, dtype=dtype), ints(5, hid, k, dtype=dtype), ints(6, n, hid, dtype=dtype)
+    bg, bu, bd = ints(7, hid, dtype=dtype), ints(8, hid, dtype=dtype), ints(9, n, dtype=dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd, bg, bu, bd)]
+    y = A.gated_ffn(*leaves, r, act=None)
+    got = torch.autograd.grad(y, leaves, dy)
+    g, u, dh = exact(x, wg.t()) + bg.double(), exact(x, wu.t()) + bu.double(), exact(dy, wd)
+    h, dg, du = ((a * b).to(dtype).double() for a, b in ((g, u), (dh, u), (dh, g)))
+    assert torch.equal(y.detach(), (exact(h, wd.t()) + bd.double() + r.double()).to(dtype))
+    want = (exact(dg, wg) + exact(du, wu), exact(dg.t(), x), exact(du.t(), x), exact(dy.t(), h), dg.sum(0), du.sum(0), dy.double().sum(0))
+    for name, a, b in zip(('dx', 'dwg', 'dwu', 'dwd', 'dbg', 'dbu', 'dbd'), got, want):
+        assert torch.equal(a, b.to(dtype)), name
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,width', [(1, 8), (129, 8), (300001, 8), (40003, 64), (40003, 256), (40003, 512), (40003, 1024), (5001, 2048), (3001, 4096), (2501, 8192)])
+def test_layer_norm_weight_gradients_are_exact(dtype, rows, width):
+    """rows of as many +1 as -1 have mean 0 and, at a width that is a power of two, variance 1: n = x, and with eps = 0 and integers for dy the
+    weight's gradient sum dy x and the bias's sum dy are integers, rounded once"""
+    from arcnerf_amd.ops import autograd as A
+    half = torch.rand(rows, width, generator=torch.Generator(device='cuda').manual_seed(1), device='cuda').argsort(1) < width // 2
+    x = torch.where(half, 1.0, -1.0).to(dtype)
+    dy = ints(2, rows, width, dtype=dtype)
+    w, b = torch.ones(width, dtype=dtype, device='cuda', requires_grad=True), torch.zeros(width, dtype=dtype, device='cuda', requires_grad=True)
+    y = A.layer_norm(x, w, b, eps=0.0)
+    assert torch.equal(y.detach(), x)
+    dw, db = torch.autograd.grad(y, [w, b], dy)
+    assert torch.equal(dw, (dy.double() * x.double()).sum(0).to(dtype)) and torch.equal(db, dy.double().sum(0).to(dtype))
+
+
+# ---- the 256-wide tiles of the 16-bit types ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize('rows,k,n,act', [(66000, 264, 264, 'silu'), (65537, 256, 256, 'gelu'), (33100, 520, 520, 'softplus'), (33100, 328, 776, None)])
+def test_dense_256_wide(dtype, rows, k, n, act):
+    """more than 256 tiles of 256 x 256 with a reduction of 256 or more: rows, features and reduction that end inside a tile or a step"""
+    from test_gpu_ffn import check_dense
+    check_dense(rows, k, n, dtype, act)
+
+
+@pytest.mark.parametrize('dtype', TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize('rows,k,hid,n,act', [(33000, 264, 520, 264, 'silu'), (32900, 256, 256, 72, 'gelu')])
+def test_gated_256_wide(dtype, rows, k, hid, n, act):
+    """the same of the gated block, whose backward has tiles of 128 features x 192 rows and a second reduction over n"""
+    from test_gpu_ffn import check_gated
+    check_gated(rows, k, hid, n, dtype, act)
+
+
+def test_256_wide_strided_rows():
+    """a pitch of whole 16-byte packs keeps the direct loads; one of single elements does not: the same results, bit for bit where the tiles agree, and
+    what lies between the rows is not touched"""
+    from arcnerf_amd.ops import functional as F
+    rows, k, n = 66001, 264, 264
+    x, w, dz = ints(1, rows, k, dtype=torch.bfloat16), ints(2, n, k, dtype=torch.bfloat16), ints(3, rows, n, dtype=torch.bfloat16)
+    want = (exact(x, w.t()).bfloat16(), exact(dz, w).bfloat16(), exact(dz.t(), x).bfloat16())
+    for pitch in (8, 3):
+        wx, wz = (torch.full((rows, t.shape[1] + pitch), float('nan'), dtype=torch.bfloat16, device='cuda') for t in (x, dz))
+        wx[:, :k], wz[:, :n] = x, dz
+        got = (F.dense_fwd(wx[:, :k], w), F.dense_dx(wz[:, :n], w), F.dense_dw(wz[:, :n], wx[:, :k])[0])
+        for name, a, b in zip(('y', 'dx', 'dw'), got, want):
+            assert torch.equal(a, b), (pitch, name)
+        assert torch.isnan(wx[:, k:]).all() and torch.isnan(wz[:, n:]).all()
+
+
+# ---- relu at pre-activations that are never zero ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,hid,n', [(50, 24, 40, 24), (8301, 130, 260, 136)])
+def test_relu_off_zero(dtype, rows, k, hid, n):
+    """x in halves, weights in quarters: the products are eighths and a bias of 1/16 keeps every sum off zero, exactly in every type"""
+    from arcnerf_amd.ops import autograd as A
+    from test_gpu_ffn import close, dense_bounds, gated_bounds, gated_inputs
+    p, dy = gated_inputs(rows, k, hid, n, dtype)
+    p['x'], p['wg'] = (p['x'] * 2).round().clamp(-3, 3) / 2, (p['wg'] * 4 * k ** 0.5).round().clamp(-2, 2) / 4
+    p['bg'] = torch.full_like(p['bg'], 0.0625)
+    q = {name: t.double() for name, t in p.items()}
+    assert (q['x'] @ q['wg'].t() + q['bg']).abs().min().item() >= 0.0625
+    d = {name: t.cuda().requires_grad_(True) for name, t in p.items()}
+    order = ('x', 'wg', 'wu', 'wd', 'bg', 'bu', 'bd', 'r')
+    want = gated_bounds(*(q[name] for name in order), dy.double(), 'relu', 1.0, dtype)
+    y = A.gated_ffn(*(d[name] for name in order), act='relu')
+    close(y, *want['y'], 'y')
+    for name, g in zip(order[:7], torch.autograd.grad(y, [d[name] for name in order[:7]], dy.cuda())):
+        close(g, *want['d' + name], 'd' + name)
+    r, dh = torch.zeros(rows, hid, dtype=torch.float64), (dy[:, :1] + torch.zeros(rows, hid, dtype=dtype))
+    want = dense_bounds(q['x'], q['wg'], q['bg'], r, dh.double(), 'relu', 1.0, dtype)
+    y = A.linear_act_residual(d['x'], d['wg'], d['bg'], act='relu')
+    close(y, *want['y'], 'dense y')
+    for key, g in zip(('dx', 'dw', 'db'), torch.autograd.grad(y, [d['x'], d['wg'], d['bg']], dh.cuda())):
+        close(g, *want[key], 'dense ' + key)
