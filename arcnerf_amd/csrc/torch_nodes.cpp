@@ -50,6 +50,10 @@ Tensor fresh(at::IntArrayRef shape, const Tensor &like, at::ScalarType type) {
 Tensor fresh(at::IntArrayRef shape, const Tensor &like) { return fresh(shape, like, like.scalar_type()); }
 Tensor scratch_floats(int64_t n, const Tensor &like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 
+// t with its numbers in memory as they are (the imaginary part of a conjugate is a view that says "negated")
+Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor packed(const Tensor &t) { return t.defined() ? plain(t).contiguous() : t; }
+
 // (..., width) as rows: a column slice of a wider buffer as it is, anything else contiguous
 struct Rows {
     Tensor t;
@@ -62,13 +66,13 @@ Rows rows_of(const char *name, const Tensor &t, int64_t width, const Tensor &lik
     TORCH_CHECK(t.scalar_type() == like.scalar_type() && t.device() == like.device(), "arcnerf_amd: ", name, " is ", t.scalar_type(), " on ", t.device(),
                 ", not ", like.scalar_type(), " on ", like.device());
     Rows r;
-    r.t = t;
-    if (t.dim() == 2 && (t.stride(1) == 1 || width == 1) && (t.stride(0) >= width || t.size(0) <= 1)) {
-        r.n = t.size(0);
-        r.ld = r.n > 1 ? t.stride(0) : width;
+    r.t = plain(t);
+    if (r.t.dim() == 2 && (r.t.stride(1) == 1 || width == 1) && (r.t.stride(0) >= width || r.t.size(0) <= 1)) {
+        r.n = r.t.size(0);
+        r.ld = r.n > 1 ? r.t.stride(0) : width;
         return r;
     }
-    r.t = t.contiguous();
+    r.t = r.t.contiguous();
     r.n = r.t.numel() / width;
     r.ld = width;
     return r;
@@ -80,7 +84,7 @@ Tensor param(const char *name, const Tensor &t, at::IntArrayRef shape, const Ten
     TORCH_CHECK(t.sizes() == shape && t.device() == like.device() && (t.scalar_type() == like.scalar_type() || (or_f32 && t.scalar_type() == at::kFloat)),
                 "arcnerf_amd: ", name, " must be ", shape, " ", like.scalar_type(), or_f32 ? " or float32" : "", " on ", like.device(), ", got ", t.sizes(), " ",
                 t.scalar_type(), " on ", t.device());
-    return t.contiguous();
+    return packed(t);
 }
 const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *out_ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -193,7 +197,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             return first_order(std::move(out), graph, "layer_norm", {x, w, g[0]});
         }
         const int dt = type_code(x, "x");
-        const Tensor wc = w.defined() ? w.contiguous() : w;
+        const Tensor wc = packed(w);
         const int64_t nf = want_dw || want_db ? arcn_layer_norm_bwd_scratch_floats(r.n, (int)C, dt) : 0;
         const Tensor scratch = nf ? scratch_floats(nf, x) : Tensor();
         Launch go(x);
@@ -248,7 +252,7 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
         at::NoGradGuard no_grad;
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], b = saved[2];
-        const Tensor w = saved[1].contiguous();
+        const Tensor w = packed(saved[1]);
         const int64_t N = w.size(0), K = w.size(1), act = ctx->saved_data["act"].toInt();
         const Needs need(ctx);
         const bool want_dx = need(0), want_dw = need(1), want_db = need(2);
@@ -261,7 +265,7 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
             Launch go(x);
             if (act != ARCN_ACT_NONE) {
                 const Rows dy = dz;
-                const Tensor bc = b.defined() ? b.contiguous() : b;
+                const Tensor bc = packed(b);
                 dz.t = fresh({r.n, N}, x);
                 dz.ld = N;
                 if (want_dx) out[0] = fresh(x.sizes(), x);
@@ -318,7 +322,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         at::NoGradGuard no_grad;
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &h = saved[6];
-        const Tensor wg = saved[1].contiguous(), wu = saved[2].contiguous(), wd = saved[3].contiguous();
+        const Tensor wg = packed(saved[1]), wu = packed(saved[2]), wd = packed(saved[3]);
         const int64_t H = wg.size(0), K = wg.size(1), N = wd.size(0);
         const Needs need(ctx);
         const int dt = type_code(x, "x");
@@ -333,7 +337,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         }
         const bool inner_w = need(1) || need(2), inner_b = need(4) || need(5);
         if (need(0) || inner_w || inner_b) {
-            const Tensor bg = saved[4].defined() ? saved[4].contiguous() : saved[4], bu = saved[5].defined() ? saved[5].contiguous() : saved[5];
+            const Tensor bg = packed(saved[4]), bu = packed(saved[5]);
             Rows dgu;
             dgu.t = fresh({r.n, 2 * H}, x);
             dgu.n = r.n;

@@ -1216,6 +1216,7 @@ def _ffn_rows(name, t, width=None, like=None):
             raise RuntimeError('arcnerf_amd: {} has {} rows, not {}'.format(name, t.shape[0], like.shape[0]))
     if t.shape[1] < 1:
         raise RuntimeError('arcnerf_amd: {} has no columns'.format(name))
+    t = t.resolve_neg()
     if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
         return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
     t = t.contiguous()
@@ -1228,7 +1229,7 @@ def _ffn_param(name, t, shape, like, types=None):
     if tuple(t.shape) != tuple(shape) or t.device != like.device or t.dtype not in (types or (like.dtype,)):
         raise RuntimeError('arcnerf_amd: {} must be {} {} on {}, got {} {} on {}'.format(
             name, tuple(shape), ' / '.join(str(d) for d in (types or (like.dtype,))), like.device, tuple(t.shape), t.dtype, t.device))
-    return t.contiguous()
+    return t.resolve_neg().contiguous()
 
 
 _SAME_DEVICE = contextlib.nullcontext()

@@ -401,3 +401,35 @@ def test_relu_off_zero(dtype, rows, k, hid, n):
     close(y, *want['y'], 'dense y')
     for key, g in zip(('dx', 'dw', 'db'), torch.autograd.grad(y, [d['x'], d['wg'], d['bg']], dh.cuda())):
         close(g, *want[key], 'dense ' + key)
+
+
+# ---- tensors whose numbers are not what memory holds ----------------------------------------------------------------------------------------
+def negated(t):
+    """-t as a view that is negated on reading, as the imaginary part of a conjugate is"""
+    v = torch.complex(torch.zeros_like(t), t).conj().imag
+    assert v.is_neg() and torch.equal(v, -t)
+    return v
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'linear_act_residual without act', 'gated_ffn'])
+def test_negated_views(name):
+    """any operand, and the gradient that comes in, as a view with its sign in the tensor and not in memory"""
+    fn, t = small_calls()[name]
+    dy = leaf(30, 40, 16).detach()
+    for k in list(t) + ['dy']:
+        results = []
+        for sign in (lambda v: -v, negated):
+            at = {j: (sign(v.detach()) if j == k else v.detach()).requires_grad_(True) for j, v in t.items()}
+            y = fn(at)
+            with torch.no_grad():
+                assert torch.equal(fn(at), y)
+            results.append((y.detach(),) + torch.autograd.grad(y, list(at.values()), sign(dy) if k == 'dy' else dy))
+        same(*results)
+
+
+def test_negated_views_in_the_calls_without_autograd():
+    from arcnerf_amd.ops import functional as F
+    x, dy, w, b = (leaf(k, *s).detach() for k, s in enumerate([(40, 16), (40, 24), (24, 16), (24,)]))
+    nx, nw, nb, ndy = (negated(t) for t in (x, w, b, dy))
+    same((F.dense_fwd(nx, nw, nb, ndy, 'silu'), F.layer_norm_fwd(nx), F.dense_dx(ndy, nw)) + F.dense_dw(ndy, nx, True),
+         (F.dense_fwd(-x, -w, -b, -dy, 'silu'), F.layer_norm_fwd(-x), F.dense_dx(-dy, -w)) + F.dense_dw(-dy, -x, True))
