@@ -5,6 +5,8 @@
 // 20011 x 319 f16, forward + backward: 48 us of kernels, 143 us a pass from Python nodes), most of it in the backward, which the engine runs
 // on a thread of its own that has to take the interpreter lock.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -131,7 +133,9 @@ bool needs_graph(std::initializer_list<const Tensor *> ts) {
 // The kernels are launched on raw pointers: a tangent would be dropped without a word, and a trace would record the allocation of a result and
 // nothing that fills it.
 void refuse_untracked(std::initializer_list<const Tensor *> ts, const char *what) {
-    TORCH_CHECK(!torch::jit::tracer::isTracing(), "arcnerf_amd: ", what, " cannot be traced (torch.jit.trace)");
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() &&
+                    !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
+                "arcnerf_amd: ", what, " cannot be traced (torch.jit.trace, make_fx)");
     for (const Tensor *t : ts)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "arcnerf_amd: ", what, " has no forward-mode derivative");
 }

@@ -846,9 +846,9 @@ def linear(x, weight, bias=None, keep_pad=False):
 # ------------------------------------------------------------------------------------------------------------------------------------
 # Residual feed-forward layers, float32 / bfloat16 / float16 (csrc/norm.hip, csrc/dense.hpp; the nodes are csrc/torch_nodes.cpp, which also
 # checks shapes, types and devices and raises RuntimeError).  First order: differentiating a gradient again raises, and so do a tensor with a
-# forward-mode tangent and torch.jit.trace.  A backward pass keeps the inputs only (layer norm: and its rows' statistics; the gated block: and the product of its
-# gate).  Calls may be captured into a graph, backward passes too (torch.autograd.grad; as for every torch operator, no eager graph of the
-# same leaves may be alive then).  CPU tensors (host-side tests of the modules) go to torch, as in `linear`.
+# forward-mode tangent and tracing (torch.jit.trace, make_fx).  A backward pass keeps the inputs only (layer norm: and its rows' statistics; the
+# gated block: and the product of its gate).  Calls may be captured into a graph, backward passes too (torch.autograd.grad; as for every torch
+# operator, no eager graph of the same leaves may be alive then).  CPU tensors (host-side tests of the modules) go to torch, as in `linear`.
 # ------------------------------------------------------------------------------------------------------------------------------------
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of x: (x - mean) / sqrt(var + eps) * weight + bias.  x float32, bfloat16 or float16; weight and

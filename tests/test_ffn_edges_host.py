@@ -109,3 +109,13 @@ def test_backward_products_take_what_a_gated_forward_takes(nodes):
     for bad in (0, -1, -(1 << 31)):
         assert lib.arcn_dense_dx(n, 1, n, n, n, 0, 0, bad, 1, n) == -1
         assert lib.arcn_dense_dw_scratch_floats(1, bad, 1, 0) == 0
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+@pytest.mark.parametrize('how', [dict(tracing_mode='real'), dict(tracing_mode='real', pre_dispatch=True)], ids=['', 'pre-dispatch'])
+def test_a_trace_into_a_graph_module_is_refused(nodes, name, how):
+    """it would record the allocation of a result and nothing that fills it"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, ops = node_calls(nodes)[name]
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        make_fx(call, **how)(*ops)

@@ -433,3 +433,23 @@ def test_negated_views_in_the_calls_without_autograd():
     nx, nw, nb, ndy = (negated(t) for t in (x, w, b, dy))
     same((F.dense_fwd(nx, nw, nb, ndy, 'silu'), F.layer_norm_fwd(nx), F.dense_dx(ndy, nw)) + F.dense_dw(ndy, nx, True),
          (F.dense_fwd(-x, -w, -b, -dy, 'silu'), F.layer_norm_fwd(-x), F.dense_dx(-dy, -w)) + F.dense_dw(-dy, -x, True))
+
+
+@pytest.mark.parametrize('name', ['layer_norm', 'linear_act_residual', 'gated_ffn'])
+def test_transforms_raise_or_are_right(name):
+    """traces into a graph module are refused, and so are batched and functional derivatives (by torch); other modes see the calls that are made"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    fn, t = small_calls()[name]
+    d = {j: v.detach() for j, v in t.items()}
+    call = lambda x: fn(dict(d, x=x))
+    x = d['x']
+    for refused in (lambda: make_fx(call)(x), lambda: make_fx(call, pre_dispatch=True)(x), lambda: make_fx(call, tracing_mode='fake')(x),
+                    lambda: torch.func.vmap(call)(torch.stack([x, x])), lambda: torch.func.grad(lambda v: call(v).sum())(x), lambda: torch.func.functionalize(call)(x),
+                    lambda: torch.autograd.grad(fn(t), t['x'], torch.ones(2, 40, 16, device='cuda'), is_grads_batched=True)):
+        with pytest.raises(RuntimeError):
+            refused()
+    want = call(x)
+    with FlopCounterMode(display=False):
+        assert torch.equal(call(x), want)
+    assert torch.equal(call(x), want)
