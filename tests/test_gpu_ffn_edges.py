@@ -453,3 +453,43 @@ def test_transforms_raise_or_are_right(name):
     with FlopCounterMode(display=False):
         assert torch.equal(call(x), want)
     assert torch.equal(call(x), want)
+
+
+# ---- infinities and NaN stay in their rows --------------------------------------------------------------------------------------------------
+def rows_apart(fn, x, dy, bad_rows):
+    """results of every row but the bad ones are, bit for bit, those without them"""
+    out = []
+    for values in ((), (float('nan'), float('inf'), -float('inf'))):
+        t = x.clone()
+        for k, v in enumerate(values):
+            t[bad_rows[k], k % x.shape[1]] = v
+        t.requires_grad_(True)
+        y = fn(t)
+        out.append((y.detach(), torch.autograd.grad(y, t, dy)[0]))
+    keep = torch.ones(x.shape[0], dtype=torch.bool, device='cuda')
+    keep[bad_rows] = False
+    for name, a, b in zip(('y', 'dx'), *out):
+        assert torch.isfinite(a).all() and torch.equal(a[keep], b[keep]), name
+    return out[1]
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('width', [3, 20, 64, 100, 256, 319, 512, 1000, 2048, 4096, 8192, 8200])
+def test_layer_norm_keeps_rows_apart(dtype, width):
+    from arcnerf_amd.ops import autograd as A
+    rows = 70
+    x, dy, w, b = (leaf(k, *s, dtype=dtype).detach() for k, s in enumerate([(rows, width), (rows, width), (width,), (width,)]))
+    y, dx = rows_apart(lambda t: A.layer_norm(t, w, b), x, dy, [5, 17, 69])
+    assert all(torch.isnan(t[r]).all() for t in (y, dx) for r in (5, 17, 69))
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,n', [(20, 24, 13), (300, 45, 21), (16400, 24, 13), (33001, 129, 130), (66000, 264, 264)])
+def test_dense_and_gated_keep_rows_apart(dtype, rows, k, n):
+    from arcnerf_amd.ops import autograd as A
+    x, dy, r = (leaf(j, rows, s, dtype=dtype).detach() for j, s in enumerate((k, n, n)))
+    w, b, wd = leaf(4, n, k, dtype=dtype, scale=k ** -0.5).detach(), leaf(5, n, dtype=dtype).detach(), leaf(6, n, n, dtype=dtype, scale=n ** -0.5).detach()
+    bad = [5, 17, rows - 1]
+    for act in ('silu', 'gelu', 'softplus', 'relu', 'sigmoid'):
+        rows_apart(lambda t: A.linear_act_residual(t, w, b, r, act=act), x, dy, bad)
+        rows_apart(lambda t: A.gated_ffn(t, w, w, wd, b, b, b, r, act=act), x, dy, bad)
