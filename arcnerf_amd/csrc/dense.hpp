@@ -384,8 +384,8 @@ struct DenseArgs {
 };
 
 // blockIdx -> tile: workgroups are dealt to the 8 XCDs in turn, so each XCD gets a contiguous range of tiles and the tiles that share
-// their J rows (the large operand) meet in one L2
-__device__ __forceinline__ uint32_t xcd_tile() { return (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
+// their J rows (the large operand) meet in one L2 (gridDim.x is a multiple of 8; y: wide_grid)
+__device__ __forceinline__ uint32_t xcd_tile() { return blockIdx.y * gridDim.x + (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
 
 // the 8 consecutive features that a lane ends up with of a pair of MFMA tiles (every lane takes part)
 __device__ __forceinline__ void swap8(f4v a, f4v b, float *v) {
@@ -963,11 +963,11 @@ static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
     const bool big = count(128, 128) >= 256 && !one_step;
     const int bi = wide ? 256 : big ? 128 : 64, bj = wide ? (MODE == kGatedBwd ? 192 : 256) : bi;
     const int64_t grid = ceil_div<int64_t>(count(bi, bj), 8) * 8;
-    if (grid > 0x7fffffff) return einval("dense: too many tiles for one launch");
+    if (grid > 0xff000000) return einval("dense: too many tiles for one launch");      // (tile numbers have 32 bits)
     p.tiles_i = (uint32_t)ceil_div<int64_t>(oi, bi);
     p.tiles_j = (uint32_t)ceil_div<int64_t>(p.j.n_out, bj);
     p.tiles = (uint32_t)count(bi, bj);
-#define ARCN_DK(WI_, WJ_, MI_, NJ_, A_) hipLaunchKernelGGL((dense_kernel<T, MODE, WI_, WJ_, MI_, NJ_, A_>), dim3((unsigned)grid), dim3(64 * WI_ * WJ_), 0, st, p)
+#define ARCN_DK(WI_, WJ_, MI_, NJ_, A_) hipLaunchKernelGGL((dense_kernel<T, MODE, WI_, WJ_, MI_, NJ_, A_>), wide_grid(grid), dim3(64 * WI_ * WJ_), 0, st, p)
     if constexpr (sizeof(T) == 2) {
         if (wide) ARCN_DK(2, 4, 8, (MODE == kGatedBwd ? 3 : 4), true);
         else if (big && async) ARCN_DK(2, 2, 4, 4, true);

@@ -5,6 +5,12 @@
 
 namespace arcn {
 
+// A launch has fewer than 2^32 threads along one dimension (2^33 were cut short here without an error): many workgroups lie in rows of 2^21.
+static inline dim3 wide_grid(int64_t blocks) {
+    const int64_t row = 1 << 21;
+    return blocks <= row ? dim3((unsigned)blocks) : dim3((unsigned)row, (unsigned)ceil_div<int64_t>(blocks, row));
+}
+
 // A workgroup sums E elements; 1024 / E threads share an element's partials, eight loads in flight each, and meet in LDS.  The elements
 // are few and the partials many (a 64 x 64 weight gradient of 10^5 rows: 4096 elements of 390 partials): one thread per element would walk
 // them alone, 600 ns a load (59 us there, 6 with E = 16).
@@ -15,7 +21,7 @@ sum_partials_kernel(const float *__restrict__ partial, int n_part, int64_t n_a, 
     constexpr int SHARES = 1024 / E;
     __shared__ float lds[SHARES][E + 1];
     const int le = threadIdx.x % E, share = threadIdx.x / E;
-    const int64_t e = (int64_t)blockIdx.x * E + le, stride = n_a + n_b;
+    const int64_t e = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * E + le, stride = n_a + n_b;
     float s[8] = {};
     if (e < stride) {
         int p = share;
@@ -46,7 +52,7 @@ template <typename T>
 static inline void sum_partials(const float *partial, int n_part, int64_t n_a, int64_t n_b, T *a, T *b, hipStream_t st) {
     const int64_t n = n_a + n_b;
 #define ARCN_SP(E_) \
-    hipLaunchKernelGGL((sum_partials_kernel<T, E_>), dim3((unsigned)ceil_div<int64_t>(n, E_)), dim3(1024), 0, st, partial, n_part, n_a, n_b, a, b)
+    hipLaunchKernelGGL((sum_partials_kernel<T, E_>), wide_grid(ceil_div<int64_t>(n, E_)), dim3(1024), 0, st, partial, n_part, n_a, n_b, a, b)
     if (n_part <= 8) ARCN_SP(1024);      // (nothing to share: 2 M elements of 4 partials 12 us, 26 with E = 256)
     else if (n <= 8192) ARCN_SP(16);
     else if (n <= 131072) ARCN_SP(64);

@@ -493,3 +493,41 @@ def test_dense_and_gated_keep_rows_apart(dtype, rows, k, n):
     for act in ('silu', 'gelu', 'softplus', 'relu', 'sigmoid'):
         rows_apart(lambda t: A.linear_act_residual(t, w, b, r, act=act), x, dy, bad)
         rows_apart(lambda t: A.gated_ffn(t, w, w, wd, b, b, b, r, act=act), x, dy, bad)
+
+
+# ---- more than 2^31 rows --------------------------------------------------------------------------------------------------------------------
+def test_more_rows_than_a_launch_has_threads():
+    """2^31 + 77 rows of one 16-bit number, more than 2^32 threads along a grid's first dimension where 64 rows have a workgroup of 256: every row
+    of the results is there, and a sum over the rows holds the last ones (x is zero but for 9 rows)"""
+    from arcnerf_amd.ops import functional as F
+    rows = (1 << 31) + 77
+    x = torch.empty(rows, 1, dtype=torch.bfloat16, device='cuda')
+    for a in range(0, rows, 1 << 28):
+        x[a:a + (1 << 28)].random_(1, 100)
+    one = torch.ones(1, 1, dtype=torch.bfloat16, device='cuda')
+    assert torch.equal(F.dense_fwd(x, one, act='relu'), x)
+    assert torch.equal(F.dense_dz(x, one, None, x, 'relu'), x)
+    assert torch.equal(F.dense_dx(x, one), x)
+    assert torch.equal(F.gated_fwd(x, torch.zeros_like(one), one, b_gate=one[0], act=None), x)
+    assert torch.equal(F.gated_bwd(x, torch.zeros_like(one), one, one[0], None, x, one, act=None)[:, 1:], x)      # du = dy
+    y = F.layer_norm_fwd(x, None, one[0])
+    assert y.min().item() == 1 and y.max().item() == 1
+    del y
+    at = torch.tensor([0, 1, 77777, 1 << 30, (1 << 31) - 1, 1 << 31, rows - 40, rows - 2, rows - 1], device='cuda')
+    few = torch.zeros_like(x)
+    few[at] = torch.tensor([1, 2, 4, 8, 16, 32, 64, 128, 256], device='cuda').bfloat16()[:, None]
+    ones = torch.ones_like(x)
+    dw, db = F.dense_dw(few, ones, want_db=True)
+    assert dw.item() == 512 and db.item() == 512       # 511, rounded to 8 bits
+    assert F.dense_dw(ones, few)[0].item() == 512
+
+
+def test_weight_gradient_of_more_elements_than_a_launch_has_threads():
+    """65544 x 65536 weights, more than 2^32: the outer product of one row, exact"""
+    from arcnerf_amd.ops import functional as F
+    n, k = 65544, 65536
+    dz, x = ints(1, 1, n, dtype=torch.bfloat16), ints(2, 1, k, dtype=torch.bfloat16)
+    dw, db = F.dense_dw(dz, x, want_db=True)
+    assert torch.equal(db, dz[0])
+    for a in range(0, n, 8192):
+        assert torch.equal(dw[a:a + 8192], dz[0, a:a + 8192, None] * x)
