@@ -11,8 +11,9 @@
 // Nothing of the forward pass but its inputs (and h) is kept for the backward: a pre-activation is computed again in the tile that needs
 // its slope, in f32, where a saved one would have been rounded to the layer's type and cost its bytes twice (2 K operations per 4 bytes:
 // at K = 256 a tile computes it faster than HBM would return it).  The gated backward computes g, u AND dh of a tile in registers; only
-// dg and du, each rounded once, are written.  (That rounding, and h's, are the 16-bit types' only ones between a call's inputs and its
-// results: dx, dW and the bias sums are made from the rounded values, which costs them as much again as their own rounding, 1.4 x in all.)
+// dg and du, each rounded once, are written.  (That rounding, and h's and dz's, are the 16-bit types' only ones between a call's inputs and
+// its results: dx and dW are made from the rounded values, which costs them as much again as their own rounding, 1.4 x in all; in f32 these
+// tensors would be twice the traffic and the products three times the operations.  The bias gradients are sums of the values before that.)
 //
 // f32 operands are split into three bf16 planes on their way into LDS, x = hi + mid + lo, and six products (hi hi, hi mid, mid hi, hi lo,
 // lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  416 TFLOP/s of f32-accurate products against 157
@@ -377,6 +378,10 @@ struct DenseArgs {
     int64_t ld_out2;
     float *partial;          // kDenseDw: [slab][n_j * n_i (+ n_j column sums of j)]
     int want_sums;
+    // Column sums of dz (dg | du) before they are rounded, 16-bit types: [n_sums][features], a row per workgroup of rows.  Written by kDenseDz,
+    // kGatedBwd and dense_dz_dx_kernel (or NULL), read by kDenseDw in place of its own sums of j (or NULL).
+    float *sums;
+    int64_t n_sums;
     int act;
     float beta, inv_beta;
     uint32_t tiles_i, tiles_j, tiles;  // tiles: of the whole product (times the slabs)
@@ -395,6 +400,14 @@ __device__ __forceinline__ void swap8(f4v a, f4v b, float *v) {
         v[r] = __builtin_bit_cast(float, (uint32_t)sw[0]);
         v[4 + r] = __builtin_bit_cast(float, (uint32_t)sw[1]);
     }
+}
+
+// the sum over the 16 lanes of a row (the 16 rows of an MFMA tile), the same value in each of them
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp_take<0xB1>(0.f, v);
+    v += dpp_take<0x4E>(0.f, v);
+    v += dpp_take<0x141>(0.f, v);
+    return v + dpp_take<0x140>(0.f, v);
 }
 
 // ASYNC: operands straight from memory to LDS (Tile::copy; launch_tiles checks what it needs)
@@ -440,7 +453,8 @@ dense_kernel(const DenseArgs<T> p) {
     float add_sums[SUM_ADD ? 8 : 1] = {};
 #pragma unroll
     for (int n = 0; n < (SUM_MMA ? NJ : 1); ++n) sums[n] = f4v{0.f, 0.f, 0.f, 0.f};
-    const bool my_sums = MODE == kDenseDw && p.want_sums && i0 == 0 && (wi == 0 || SUM_ADD);   // wave-uniform
+    const bool given_sums = SUM_MMA && p.want_sums && i0 == 0 && p.sums;
+    const bool my_sums = MODE == kDenseDw && p.want_sums && i0 == 0 && (wi == 0 || SUM_ADD) && !given_sums;   // wave-uniform
 
     // after the swap a lane holds 8 features of a pair of tiles from 32 pr + f8, row o
     const int g = lane >> 4, o = lane & 15, f8 = 16 * (g & 1) + 8 * (g >> 1);
@@ -581,6 +595,18 @@ dense_kernel(const DenseArgs<T> p) {
     }
 
     // ---- epilogue -----------------------------------------------------------------------------------------------------------------------
+    // the column sums of what is stored, not rounded: a wave's rows in registers, the WJ waves of a tile in LDS ([wave][column of out])
+    constexpr bool SUMS = (MODE == kDenseDz || MODE == kGatedBwd) && sizeof(T) == 2;
+    constexpr int SUM_COLS = GATED ? 2 * OUT_I : OUT_I;
+    float *const red = reinterpret_cast<float *>(lds);      // behind the products' last barrier
+    auto keep_sums = [&](float *v, int col) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = sum16(v[e]);
+        if (o == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) red[wj * SUM_COLS + col + e] = v[e];
+        }
+    };
     auto pair8 = [&](auto &c, int pr, int n, float *v) { swap8(c[2 * pr][n], c[2 * pr + 1][n], v); };
     auto bias8 = [&](const T *b, int64_t i, float *v) {
 #pragma unroll
@@ -601,6 +627,25 @@ dense_kernel(const DenseArgs<T> p) {
             }
             if (SUM_MMA && my_sums && g == 0 && j < p.j.n_out) part[p.i.n_out * p.j.n_out + j] = sums[n][0];
         }
+        if constexpr (SUM_MMA) {
+            if (given_sums) {      // the slab's share of them: THREADS / BJ threads to a column
+                const int64_t lo = p.n_sums * slab / p.slabs, hi = p.n_sums * (slab + 1) / p.slabs, j = j0 + tid % BJ;
+                float v = 0.f;
+                if (j < p.j.n_out) {
+#pragma unroll 8
+                    for (int64_t k = lo + tid / BJ; k < hi; k += THREADS / BJ) v += p.sums[k * p.j.n_out + j];
+                }
+                float *f = reinterpret_cast<float *>(lds);      // behind the product's last barrier
+                f[tid] = v;
+                __syncthreads();
+                if (tid < BJ && j < p.j.n_out) {
+                    v = 0.f;
+#pragma unroll
+                    for (int k = 0; k < THREADS / BJ; ++k) v += f[k * BJ + tid];
+                    part[p.i.n_out * p.j.n_out + j] = v;
+                }
+            }
+        }
         if (SUM_ADD && my_sums) {
             float *f = reinterpret_cast<float *>(lds);      // [thread][8]; behind the product's last barrier
 #pragma unroll
@@ -620,6 +665,7 @@ dense_kernel(const DenseArgs<T> p) {
             float bg[8], bu[8];
             bias8(p.bias, i, bg);
             bias8(p.bias2, i, bu);
+            float sg[8] = {}, su[8] = {};
 #pragma unroll
             for (int n = 0; n < NJ; ++n) {
                 const int64_t j = j0 + (wj * NJ + n) * 16 + o;
@@ -643,9 +689,20 @@ dense_kernel(const DenseArgs<T> p) {
                         gv[e] = dh[e] * (uv[e] + bu[e]) * slope;
                         uv[e] = dh[e] * a;
                     }
+                    if (SUMS && p.sums) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            sg[e] += j < p.j.n_out ? gv[e] : 0.f;
+                            su[e] += j < p.j.n_out ? uv[e] : 0.f;
+                        }
+                    }
                     store8<T>(dst, gv, left);
                     store8<T>(dst + p.i.n_out, uv, left);   // du behind dg in a row of 2 H
                 }
+            }
+            if (SUMS && p.sums) {
+                keep_sums(sg, wi * 8 * MI + 32 * pr + f8);
+                keep_sums(su, OUT_I + wi * 8 * MI + 32 * pr + f8);
             }
         }
         });
@@ -657,6 +714,7 @@ dense_kernel(const DenseArgs<T> p) {
             const int64_t i = i0 + wi * 16 * MI + 32 * pr + f8;
             float b[8];
             bias8(MODE == kDenseDx ? nullptr : p.bias, i, b);
+            float sz[8] = {};
 #pragma unroll
             for (int n = 0; n < NJ; ++n) {
                 const int64_t j = j0 + (wj * NJ + n) * 16 + o;
@@ -681,10 +739,28 @@ dense_kernel(const DenseArgs<T> p) {
                         }
                     }
                 }
+                if (SUMS && p.sums) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sz[e] += j < p.j.n_out ? v[e] : 0.f;
+                }
                 store8<T>(p.out + j * p.ld_out + i, v, j < p.j.n_out ? p.i.n_out - i : 0);
             }
+            if (SUMS && p.sums) keep_sums(sz, wi * 16 * MI + 32 * pr + f8);
         }
         });
+    }
+    if constexpr (SUMS) {
+        if (p.sums) {
+            __syncthreads();
+            for (int c = tid; c < SUM_COLS; c += THREADS) {
+                const int64_t i = i0 + c % OUT_I;
+                if (i >= p.i.n_out) continue;
+                float v = 0.f;
+#pragma unroll
+                for (int k = 0; k < WJ; ++k) v += red[k * SUM_COLS + c];
+                p.sums[(int64_t)rest * p.ld_out + (c / OUT_I) * p.i.n_out + i] = v;
+            }
+        }
     }
 }
 
@@ -773,7 +849,7 @@ template <typename T, int KS>
 __global__ void __launch_bounds__(512, 2)
 dense_dz_dx_kernel(const DenseArgs<T> p) {
     constexpr int WAVES = 8, NT = 8, ROW = KS * 4;      // NT: feature tiles of a pass; ROW: 16-byte chunks per LDS row
-    extern __shared__ __attribute__((aligned(16))) short w[];      // [N up to a multiple of 128][KS * 32], then the bias
+    extern __shared__ __attribute__((aligned(16))) short w[];      // [N up to a multiple of 128][KS * 32], the bias, if wanted the waves' sums
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, o = lane & 15, g = lane >> 4, f8 = 16 * (g & 1) + 8 * (g >> 1);
     int K = (int)p.i.n_red, N = (int)p.i.n_out;
     const int ks = (K + 31) / 32, n_pad = (N + 127) / 128 * 128;
@@ -785,6 +861,9 @@ dense_dz_dx_kernel(const DenseArgs<T> p) {
         *reinterpret_cast<u4v *>(w + 8 * (n * ROW + (c ^ swizzle(n)))) = load8<T>(p.i.a + (int64_t)(n < N ? n : 0) * p.i.ld + 8 * c, n < N ? K - 8 * c : 0).v[0];
     }
     for (int n = tid; n < n_pad; n += 64 * WAVES) bias[n] = p.bias && n < N ? p.bias[n] : (T)0.f;
+    float *const sums = reinterpret_cast<float *>(bias + n_pad), *const mine = sums + wave * n_pad;
+    if (p.sums)
+        for (int n = tid; n < WAVES * n_pad; n += 64 * WAVES) sums[n] = 0.f;
     __syncthreads();
 
     const int64_t rows = p.j.n_out, step = (int64_t)gridDim.x * WAVES * 16;
@@ -859,6 +938,15 @@ dense_dz_dx_kernel(const DenseArgs<T> p) {
                         for (int e = 0; e < 8; ++e) v[e] = n0 + 32 * pr + f8 + e < N ? v[e] : 0.f;
                     }
                     dy[pr] = Elem<T>::pack(v);      // dz from here on
+                    if (p.sums) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = sum16(live ? v[e] : 0.f);
+                        if (o == 0) {
+                            float *const at = mine + n0 + 32 * pr + f8;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) at[e] += v[e];
+                        }
+                    }
                 }
             });
 #pragma unroll
@@ -899,6 +987,15 @@ dense_dz_dx_kernel(const DenseArgs<T> p) {
             }
         }
     }
+    if (p.sums) {
+        __syncthreads();
+        for (int n = tid; n < N; n += 64 * WAVES) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k) v += sums[k * n_pad + n];
+            p.sums[(int64_t)blockIdx.x * N + n] = v;
+        }
+    }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------------
@@ -918,11 +1015,13 @@ static bool dense_stays(int64_t rows, int K, int N) {
     return sizeof(T) == 2 && K >= 8 && N >= 8 && K <= 128 && N <= 512 && rows >= kStayRows;
 }
 template <typename T>
-static int launch_dz_dx(const DenseArgs<T> &p, hipStream_t st) {
+static int launch_dz_dx(DenseArgs<T> &p, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        const int bytes = ceil_div<int>((int)p.i.n_out, 128) * 128 * (256 + 2);      // the weight's rows of 128 inputs, and the bias
+        // the weight's rows of 128 inputs, the bias, the eight waves' sums
+        const int bytes = ceil_div<int>((int)p.i.n_out, 128) * 128 * (256 + 2 + (p.sums ? 32 : 0));
         const int64_t g = ceil_div<int64_t>(p.j.n_out, 128), most = bytes <= 80 * 1024 ? 512 : 256;
-        hipLaunchKernelGGL((dense_dz_dx_kernel<T, 4>), dim3((unsigned)(g < most ? g : most)), dim3(512), bytes, st, p);
+        p.n_sums = g < most ? g : most;
+        hipLaunchKernelGGL((dense_dz_dx_kernel<T, 4>), dim3((unsigned)p.n_sums), dim3(512), bytes, st, p);
     }
     return check_launch("dense_dz");
 }
@@ -967,6 +1066,7 @@ static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
     p.tiles_i = (uint32_t)ceil_div<int64_t>(oi, bi);
     p.tiles_j = (uint32_t)ceil_div<int64_t>(p.j.n_out, bj);
     p.tiles = (uint32_t)count(bi, bj);
+    if (MODE != kDenseDw) p.n_sums = p.tiles_j;
 #define ARCN_DK(WI_, WJ_, MI_, NJ_, A_) hipLaunchKernelGGL((dense_kernel<T, MODE, WI_, WJ_, MI_, NJ_, A_>), wide_grid(grid), dim3(64 * WI_ * WJ_), 0, st, p)
     if constexpr (sizeof(T) == 2) {
         if (wide) ARCN_DK(2, 4, 8, (MODE == kGatedBwd ? 3 : 4), true);
@@ -981,20 +1081,23 @@ static int launch_tiles(DenseArgs<T> &p, hipStream_t st) {
     return check_launch("dense");
 }
 
+// rows of column sums that a kernel may write: the smallest tile has 64 rows
+static inline int64_t dense_sums_rows(int64_t rows) { return ceil_div<int64_t>(rows, 64); }
+
+// sums, n_sums: of DenseArgs; NULL or, 16-bit types, where the column sums go and how many rows of them there are
 template <typename T>
 struct DenseOps {
     static int fwd(const void *x, int64_t ld_x, const void *w, const void *b, const void *res, int64_t ld_res, void *y, int act, float beta, int64_t rows, int K, int N,
                    hipStream_t st);
-    static int dz(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, int act, float beta, int64_t rows, int K, int N,
-                  hipStream_t st);
     static int dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int64_t rows, int N, int K, hipStream_t st);
-    static int dz_dx(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, void *dx, int act, float beta, int64_t rows, int K,
-                     int N, hipStream_t st);
-    static int dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, float *scratch, int64_t rows, int N, int K, hipStream_t st);
+    static int dz_dx(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, void *dx, int act, float beta, float *sums,
+                     int64_t *n_sums, int64_t rows, int K, int N, hipStream_t st);
+    static int dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, const float *sums, int64_t n_sums, void *dw, void *db, float *scratch, int64_t rows, int N, int K,
+                  hipStream_t st);
     static int gated_fwd(const void *x, int64_t ld_x, const void *wg, const void *wu, const void *bg, const void *bu, void *h, int act, float beta, int64_t rows, int K,
                          int H, hipStream_t st);
     static int gated_bwd(const void *x, int64_t ld_x, const void *wg, const void *wu, const void *bg, const void *bu, const void *dy, int64_t ld_dy, const void *wd,
-                         void *dgu, int act, float beta, int64_t rows, int K, int H, int N, hipStream_t st);
+                         void *dgu, int act, float beta, float *sums, int64_t *n_sums, int64_t rows, int K, int H, int N, hipStream_t st);
 };
 
 }  // namespace arcn

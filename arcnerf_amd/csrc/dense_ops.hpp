@@ -34,23 +34,6 @@ int DenseOps<T>::fwd(const void *x, int64_t ld_x, const void *w, const void *b, 
 }
 
 template <typename T>
-int DenseOps<T>::dz(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, int act, float beta, int64_t rows, int K, int N,
-                    hipStream_t st) {
-    DenseArgs<T> p = {};
-    p.i = {tp<T>(w), nullptr, K, N, K, 0};
-    p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
-    p.bias = tp<T>(b);
-    p.res = tp<T>(dy);
-    p.ld_res = ld_dy;
-    p.out = static_cast<T *>(dz);
-    p.ld_out = N;
-    p.act = act;
-    p.beta = beta;
-    p.inv_beta = 1.f / beta;
-    return launch_tiles<T, kDenseDz>(p, st);
-}
-
-template <typename T>
 int DenseOps<T>::dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int64_t rows, int N, int K, hipStream_t st) {
     DenseArgs<T> p = {};
     p.i = {tp<T>(w), tp<T>(w2), K, K, N, N / 2};
@@ -61,35 +44,40 @@ int DenseOps<T>::dx(const void *dz, int64_t ld_dz, const void *w, const void *w2
 }
 
 template <typename T>
-int DenseOps<T>::dz_dx(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz_, void *dx_, int act, float beta, int64_t rows,
-                       int K, int N, hipStream_t st) {
-    if (!dx_ || !dense_stays<T>(rows, K, N)) {
-        if (int rc = dz(x, ld_x, w, b, dy, ld_dy, dz_, act, beta, rows, K, N, st)) return rc;
-        return dx_ ? dx(dz_, N, w, nullptr, dx_, rows, N, K, st) : ARCN_OK;
-    }
+int DenseOps<T>::dz_dx(const void *x, int64_t ld_x, const void *w, const void *b, const void *dy, int64_t ld_dy, void *dz, void *dx_, int act, float beta, float *sums,
+                       int64_t *n_sums, int64_t rows, int K, int N, hipStream_t st) {
     DenseArgs<T> p = {};
     p.i = {tp<T>(w), nullptr, K, N, K, 0};
     p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
     p.bias = tp<T>(b);
     p.res = tp<T>(dy);
     p.ld_res = ld_dy;
-    p.out = static_cast<T *>(dz_);
+    p.out = static_cast<T *>(dz);
     p.ld_out = N;
-    p.out2 = static_cast<T *>(dx_);
-    p.ld_out2 = K;
+    p.sums = sums;
     p.act = act;
     p.beta = beta;
     p.inv_beta = 1.f / beta;
-    return launch_dz_dx<T>(p, st);
+    const bool stays = dx_ && dense_stays<T>(rows, K, N);
+    if (stays) {
+        p.out2 = static_cast<T *>(dx_);
+        p.ld_out2 = K;
+    }
+    if (int rc = stays ? launch_dz_dx<T>(p, st) : launch_tiles<T, kDenseDz>(p, st)) return rc;
+    if (sums) *n_sums = p.n_sums;
+    return !stays && dx_ ? dx(dz, N, w, nullptr, dx_, rows, N, K, st) : ARCN_OK;
 }
 
 template <typename T>
-int DenseOps<T>::dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, float *scratch, int64_t rows, int N, int K, hipStream_t st) {
+int DenseOps<T>::dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, const float *sums, int64_t n_sums, void *dw, void *db, float *scratch, int64_t rows, int N,
+                    int K, hipStream_t st) {
     DenseArgs<T> p = {};
     p.i = {tp<T>(x), nullptr, ld_x, K, rows, 0};
     p.j = {tp<T>(dz), nullptr, ld_dz, N, rows, 0};
     p.partial = scratch;
     p.want_sums = db != nullptr;
+    p.sums = const_cast<float *>(sums);      // (read)
+    p.n_sums = n_sums;
     p.slabs = dense_dw_slabs(sizeof(T), rows, N, K);
     if (int rc = launch_tiles<T, kDenseDw>(p, st)) return rc;
     const int64_t n = (int64_t)N * K, n_db = db ? N : 0;
@@ -121,7 +109,7 @@ int DenseOps<T>::gated_fwd(const void *x, int64_t ld_x, const void *wg, const vo
 
 template <typename T>
 int DenseOps<T>::gated_bwd(const void *x, int64_t ld_x, const void *wg, const void *wu, const void *bg, const void *bu, const void *dy, int64_t ld_dy, const void *wd,
-                           void *dgu, int act, float beta, int64_t rows, int K, int H, int N, hipStream_t st) {
+                           void *dgu, int act, float beta, float *sums, int64_t *n_sums, int64_t rows, int K, int H, int N, hipStream_t st) {
     DenseArgs<T> p = {};
     p.i = {tp<T>(wg), tp<T>(wu), K, H, K, 0};
     p.j = {tp<T>(x), nullptr, ld_x, rows, K, 0};
@@ -131,10 +119,13 @@ int DenseOps<T>::gated_bwd(const void *x, int64_t ld_x, const void *wg, const vo
     p.bias2 = tp<T>(bu);
     p.out = static_cast<T *>(dgu);
     p.ld_out = 2 * (int64_t)H;
+    p.sums = sums;
     p.act = act;
     p.beta = beta;
     p.inv_beta = 1.f / beta;
-    return launch_tiles<T, kGatedBwd>(p, st);
+    if (int rc = launch_tiles<T, kGatedBwd>(p, st)) return rc;
+    if (sums) *n_sums = p.n_sums;
+    return ARCN_OK;
 }
 
 }  // namespace arcn

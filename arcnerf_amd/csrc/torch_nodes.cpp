@@ -233,12 +233,24 @@ Tensor dense_forward(const Tensor &x, const Tensor &w, const Tensor &b, const Te
     return y;
 }
 
-// dw (N, K) = dz^T x, db = column sums of dz (or undefined)
-std::pair<Tensor, Tensor> dense_dw(const Rows &dz, int64_t N, const Rows &x, int64_t K, bool want_db, int dt, void *stream) {
+// The column sums of dz, made where it is still in f32: of the 16-bit types, where a bias's gradient is wanted
+struct BiasSums {
+    Tensor t;
+    int64_t n = 0;
+    BiasSums() = default;
+    BiasSums(bool want, int64_t rows, int64_t N, const Tensor &like) {
+        if (want && like.scalar_type() != at::kFloat) t = scratch_floats(arcn_bias_sums_floats(rows, (int)N), like);
+    }
+    float *p() const { return (float *)out_ptr(t); }
+    int64_t floats() const { return t.defined() ? t.numel() : 0; }
+};
+
+// dw (N, K) = dz^T x, db = column sums of dz (or undefined), as `sums` has them or its own
+std::pair<Tensor, Tensor> dense_dw(const Rows &dz, int64_t N, const Rows &x, int64_t K, bool want_db, const BiasSums &sums, int dt, void *stream) {
     Tensor dw = fresh({N, K}, x.t), db = want_db ? fresh({N}, x.t) : Tensor();
     const int64_t nf = arcn_dense_dw_scratch_floats(x.n, (int)N, (int)K, dt);
     const Tensor scratch = scratch_floats(nf, x.t);
-    call(arcn_dense_dw(dz.p(), dz.ld, x.p(), x.ld, dw.data_ptr(), out_ptr(db), dt, scratch.data_ptr<float>(), nf, x.n, (int)N, (int)K, stream), "dense_dw");
+    call(arcn_dense_dw_sums(dz.p(), dz.ld, x.p(), x.ld, sums.p(), sums.n, dw.data_ptr(), out_ptr(db), dt, scratch.data_ptr<float>(), nf, x.n, (int)N, (int)K, stream), "dense_dw");
     return {dw, db};
 }
 
@@ -266,6 +278,7 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
             const Rows r = rows_of("x", x, K, x);
             Rows dz = rows_of("dy", g[0], N, x);
             const int dt = type_code(x, "x");
+            BiasSums sums;
             Launch go(x);
             if (act != ARCN_ACT_NONE) {
                 const Rows dy = dz;
@@ -273,15 +286,16 @@ struct LinearActResidual : torch::autograd::Function<LinearActResidual> {
                 dz.t = fresh({r.n, N}, x);
                 dz.ld = N;
                 if (want_dx) out[0] = fresh(x.sizes(), x);
-                call(arcn_dense_dz(r.p(), r.ld, ptr(w), ptr(bc), dy.p(), dy.ld, dz.t.data_ptr(), out_ptr(out[0]), dt, (int)act,
-                                   (float)ctx->saved_data["beta"].toDouble(), r.n, (int)K, (int)N, go.stream),
+                sums = BiasSums(want_db, r.n, N, x);
+                call(arcn_dense_dz_sums(r.p(), r.ld, ptr(w), ptr(bc), dy.p(), dy.ld, dz.t.data_ptr(), out_ptr(out[0]), sums.p(), sums.floats(), &sums.n, dt, (int)act,
+                                        (float)ctx->saved_data["beta"].toDouble(), r.n, (int)K, (int)N, go.stream),
                      "dense_dz");
             } else if (want_dx) {
                 out[0] = fresh(x.sizes(), x);
                 call(arcn_dense_dx(dz.p(), dz.ld, ptr(w), nullptr, out[0].data_ptr(), dt, r.n, (int)N, (int)K, go.stream), "dense_dx");
             }
             if (want_dw || want_db) {
-                auto [dw, db] = dense_dw(dz, N, r, K, want_db, dt, go.stream);
+                auto [dw, db] = dense_dw(dz, N, r, K, want_db, sums, dt, go.stream);
                 if (want_dw) out[1] = dw;
                 out[2] = db;
             }
@@ -335,7 +349,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         const Rows r = rows_of("x", x, K, x), dy = rows_of("dy", g[0], N, x);
         Launch go(x);
         if (need(3) || need(6)) {
-            auto [dw, db] = dense_dw(dy, N, rows_of("h", h, H, x), H, need(6), dt, go.stream);
+            auto [dw, db] = dense_dw(dy, N, rows_of("h", h, H, x), H, need(6), BiasSums(), dt, go.stream);
             if (need(3)) out[3] = dw;
             out[6] = db;
         }
@@ -346,15 +360,16 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
             dgu.t = fresh({r.n, 2 * H}, x);
             dgu.n = r.n;
             dgu.ld = 2 * H;
-            call(arcn_gated_bwd(r.p(), r.ld, ptr(wg), ptr(wu), ptr(bg), ptr(bu), dy.p(), dy.ld, ptr(wd), dgu.t.data_ptr(), dt, (int)ctx->saved_data["act"].toInt(),
-                                (float)ctx->saved_data["beta"].toDouble(), r.n, (int)K, (int)H, (int)N, go.stream),
+            BiasSums sums(inner_b, r.n, 2 * H, x);
+            call(arcn_gated_bwd_sums(r.p(), r.ld, ptr(wg), ptr(wu), ptr(bg), ptr(bu), dy.p(), dy.ld, ptr(wd), dgu.t.data_ptr(), sums.p(), sums.floats(), &sums.n, dt,
+                                     (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["beta"].toDouble(), r.n, (int)K, (int)H, (int)N, go.stream),
                  "gated_bwd");
             if (need(0)) {
                 out[0] = fresh(x.sizes(), x);
                 call(arcn_dense_dx(dgu.p(), dgu.ld, ptr(wg), ptr(wu), out[0].data_ptr(), dt, r.n, (int)(2 * H), (int)K, go.stream), "dense_dx");
             }
             if (inner_w || inner_b) {
-                auto [dw, db] = dense_dw(dgu, 2 * H, r, K, inner_b, dt, go.stream);
+                auto [dw, db] = dense_dw(dgu, 2 * H, r, K, inner_b, sums, dt, go.stream);
                 if (need(1)) out[1] = dw.narrow(0, 0, H);
                 if (need(2)) out[2] = dw.narrow(0, H, H);
                 if (need(4)) out[4] = db.narrow(0, 0, H);

@@ -1297,21 +1297,31 @@ def dense_fwd(x, w, bias=None, residual=None, act=None, beta=1.0):
     return y
 
 
-def dense_dz(x, w, bias, dy, act, beta=1.0, want_dx=False):
-    """dy * act'(x @ w.T + bias), the pre-activation computed again (dy itself where there is no activation); want_dx: also that @ w"""
+def _bias_sums(want, S, n, like):
+    """(where a kernel puts the column sums of what it rounds to 16 bits, their room, the host number that it sets)"""
+    nf = int(N.lib().arcn_bias_sums_floats(S, n)) if want and like.dtype != torch.float32 else 0
+    return torch.empty(nf, dtype=torch.float32, device=like.device) if nf else None, nf, C.c_int64(0)
+
+
+def dense_dz(x, w, bias, dy, act, beta=1.0, want_dx=False, want_sums=False):
+    """dy * act'(x @ w.T + bias), the pre-activation computed again (dy itself where there is no activation); want_dx: also that @ w.  want_sums: as the
+    last result also partial column sums (n, N) of it from before it was rounded to 16 bits, which dense_dw takes (None where nothing is rounded)"""
     _req(x, w, bias, dy)
     x, ld = _ffn_rows('x', x)
     (S, K), Nn, code = x.shape, w.shape[0], _dense_act(act, beta)
     w, bias = _ffn_param('weight', w, (Nn, K), x), _ffn_param('bias', bias, (Nn,), x)
     dy, ld_dy = _ffn_rows('dy', dy, Nn, like=x)
     if code == 0:
-        return (dy, dense_dx(dy, w)) if want_dx else dy
+        out = (dy, *((dense_dx(dy, w),) if want_dx else ()), *((None,) if want_sums else ()))
+        return out if len(out) > 1 else dy
     dz = _fresh((S, Nn), x.dtype, x.device)
     dx = _fresh((S, K), x.dtype, x.device) if want_dx else None
+    sums, nf, n_sums = _bias_sums(want_sums, S, Nn, x)
     with _device_of(x):
-        N.check(N.lib().arcn_dense_dz(x.data_ptr(), ld, N.ptr(w), N.ptr(bias), dy.data_ptr(), ld_dy, N.ptr(dz), N.ptr(dx), _DTYPE[x.dtype], code, float(beta), S, K, Nn,
-                                      N.stream()), 'dense_dz')
-    return (dz, dx) if want_dx else dz
+        N.check(N.lib().arcn_dense_dz_sums(x.data_ptr(), ld, N.ptr(w), N.ptr(bias), dy.data_ptr(), ld_dy, N.ptr(dz), N.ptr(dx), N.ptr(sums), nf, C.byref(n_sums),
+                                           _DTYPE[x.dtype], code, float(beta), S, K, Nn, N.stream()), 'dense_dz')
+    out = (dz, *((dx,) if want_dx else ()), *((None if sums is None else sums.view(-1, Nn)[:n_sums.value],) if want_sums else ()))
+    return out if len(out) > 1 else dz
 
 
 def dense_dx(dz, w, w2=None):
@@ -1329,8 +1339,9 @@ def dense_dx(dz, w, w2=None):
     return dx
 
 
-def dense_dw(dz, x, want_db=False):
-    """(dz (S, N).T @ x (S, K), column sums of dz or None), summed over the rows in a fixed order"""
+def dense_dw(dz, x, want_db=False, sums=None):
+    """(dz (S, N).T @ x (S, K), column sums of dz or None), summed over the rows in a fixed order.  sums: those of dense_dz / gated_bwd, of which the column
+    sums are made in place of the rounded dz"""
     _req(dz, x)
     x, ld_x = _ffn_rows('x', x)
     dz, ld = _ffn_rows('dz', dz, like=x)
@@ -1339,8 +1350,11 @@ def dense_dw(dz, x, want_db=False):
     db = _fresh((Nn,), x.dtype, x.device) if want_db else None
     nf = int(N.lib().arcn_dense_dw_scratch_floats(S, Nn, K, _DTYPE[x.dtype]))
     scratch = torch.empty(nf, dtype=torch.float32, device=x.device)
+    if sums is not None and (sums.dim() != 2 or sums.shape[1] != Nn or sums.dtype != torch.float32 or sums.device != x.device):
+        raise RuntimeError('arcnerf_amd: sums must be (n, {}) float32 on {}, got {} {} on {}'.format(Nn, x.device, tuple(sums.shape), sums.dtype, sums.device))
+    sums = None if sums is None or not want_db else sums.contiguous()
     with _device_of(x):
-        N.check(N.lib().arcn_dense_dw(dz.data_ptr(), ld, x.data_ptr(), ld_x, N.ptr(dw), N.ptr(db), _DTYPE[x.dtype], N.ptr(scratch), nf, S, Nn, K, N.stream()),
+        N.check(N.lib().arcn_dense_dw_sums(dz.data_ptr(), ld, x.data_ptr(), ld_x, N.ptr(sums), 0 if sums is None else sums.shape[0], N.ptr(dw), N.ptr(db), _DTYPE[x.dtype], N.ptr(scratch), nf, S, Nn, K, N.stream()),
                 'dense_dw')
     return dw, db
 
@@ -1359,9 +1373,9 @@ def gated_fwd(x, w_gate, w_up, b_gate=None, b_up=None, act='silu', beta=1.0):
     return h
 
 
-def gated_bwd(x, w_gate, w_up, b_gate, b_up, dy, w_down, act='silu', beta=1.0):
+def gated_bwd(x, w_gate, w_up, b_gate, b_up, dy, w_down, act='silu', beta=1.0, want_sums=False):
     """(S, 2 H) = [d gate | d up], the gradients of the two pre-activations of gated_fwd for the gradient dy (S, N) of h @ w_down (N, H).T: both
-    pre-activations and dy @ w_down are computed in the kernel"""
+    pre-activations and dy @ w_down are computed in the kernel.  want_sums: also (n, 2 H) column sums, as dense_dz has them"""
     _req(x, w_gate, w_up, b_gate, b_up, dy, w_down)
     x, ld = _ffn_rows('x', x)
     (S, K), H, Nn, code = x.shape, w_gate.shape[0], w_down.shape[0], _dense_act(act, beta)
@@ -1369,10 +1383,11 @@ def gated_bwd(x, w_gate, w_up, b_gate, b_up, dy, w_down, act='silu', beta=1.0):
     b_gate, b_up, w_down = _ffn_param('b_gate', b_gate, (H,), x), _ffn_param('b_up', b_up, (H,), x), _ffn_param('w_down', w_down, (Nn, H), x)
     dy, ld_dy = _ffn_rows('dy', dy, Nn, like=x)
     dgu = _fresh((S, 2 * H), x.dtype, x.device)
+    sums, nf, n_sums = _bias_sums(want_sums, S, 2 * H, x)
     with _device_of(x):
-        N.check(N.lib().arcn_gated_bwd(x.data_ptr(), ld, N.ptr(w_gate), N.ptr(w_up), N.ptr(b_gate), N.ptr(b_up), dy.data_ptr(), ld_dy, N.ptr(w_down), N.ptr(dgu),
-                                       _DTYPE[x.dtype], code, float(beta), S, K, H, Nn, N.stream()), 'gated_bwd')
-    return dgu
+        N.check(N.lib().arcn_gated_bwd_sums(x.data_ptr(), ld, N.ptr(w_gate), N.ptr(w_up), N.ptr(b_gate), N.ptr(b_up), dy.data_ptr(), ld_dy, N.ptr(w_down), N.ptr(dgu),
+                                            N.ptr(sums), nf, C.byref(n_sums), _DTYPE[x.dtype], code, float(beta), S, K, H, Nn, N.stream()), 'gated_bwd')
+    return (dgu, None if sums is None else sums.view(-1, 2 * H)[:n_sums.value]) if want_sums else dgu
 
 
 # ------------------------------------------------------------------------------------------------

@@ -837,12 +837,21 @@ int arcn_dense_fwd(const void *x, int64_t ld_x, const void *w, const void *bias,
  * NULL also dx (n_rows, K) = dz w, in the same kernel where the weight fits on chip */
 int arcn_dense_dz(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, void *dx, int dtype, int act,
                   float beta, int64_t n_rows, int K, int N, void *stream);
+/* The same, and the column sums of dz before it is rounded to 16 bits (the bias's gradient needs no rounded terms): sums (16-bit types; may be NULL)
+ * holds arcn_bias_sums_floats(n_rows, N) floats and receives (*n_sums, N) partial sums, which arcn_dense_dw_sums adds up.  *n_sums is a host
+ * variable, written before the call returns. */
+int64_t arcn_bias_sums_floats(int64_t n_rows, int N);
+int arcn_dense_dz_sums(const void *x, int64_t ld_x, const void *w, const void *bias, const void *dy, int64_t ld_dy, void *dz, void *dx, float *sums,
+                       int64_t sums_floats, int64_t *n_sums, int dtype, int act, float beta, int64_t n_rows, int K, int N, void *stream);
 /* dx (n_rows, K) = dz (n_rows, N) w (N, K).  w2 not NULL (N even): the weight's first N / 2 rows are w (N / 2, K), the others w2. */
 int arcn_dense_dx(const void *dz, int64_t ld_dz, const void *w, const void *w2, void *dx, int dtype, int64_t n_rows, int N, int K, void *stream);
 /* dw (N, K) = dz^T x and, unless db is NULL, db (N) = the column sums of dz.  scratch: arcn_dense_dw_scratch_floats floats. */
 int64_t arcn_dense_dw_scratch_floats(int64_t n_rows, int N, int K, int dtype);
 int arcn_dense_dw(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, void *dw, void *db, int dtype, float *scratch, int64_t scratch_floats,
                   int64_t n_rows, int N, int K, void *stream);
+/* The same with db the sum of the n_sums rows of sums (of arcn_dense_dz_sums or arcn_gated_bwd_sums; sums NULL: arcn_dense_dw) */
+int arcn_dense_dw_sums(const void *dz, int64_t ld_dz, const void *x, int64_t ld_x, const float *sums, int64_t n_sums, void *dw, void *db, int dtype,
+                       float *scratch, int64_t scratch_floats, int64_t n_rows, int N, int K, void *stream);
 /* h (n_rows, H) = act(x w_gate^T + b_gate) * (x w_up^T + b_up); w_gate and w_up (H, K), biases (H) or NULL */
 int arcn_gated_fwd(const void *x, int64_t ld_x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, void *h, int dtype, int act,
                    float beta, int64_t n_rows, int K, int H, void *stream);
@@ -851,6 +860,10 @@ int arcn_gated_fwd(const void *x, int64_t ld_x, const void *w_gate, const void *
  * w_gate, w_up) and arcn_dense_dw(dgu, x), whose (2 H, K) result is both weights' gradients, and arcn_dense_dw(dy, h). */
 int arcn_gated_bwd(const void *x, int64_t ld_x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, const void *dy, int64_t ld_dy,
                    const void *w_down, void *dgu, int dtype, int act, float beta, int64_t n_rows, int K, int H, int N, void *stream);
+/* The same, and the column sums of dgu before it is rounded, as arcn_dense_dz_sums makes them: sums holds arcn_bias_sums_floats(n_rows, 2 H) */
+int arcn_gated_bwd_sums(const void *x, int64_t ld_x, const void *w_gate, const void *w_up, const void *b_gate, const void *b_up, const void *dy, int64_t ld_dy,
+                        const void *w_down, void *dgu, float *sums, int64_t sums_floats, int64_t *n_sums, int dtype, int act, float beta, int64_t n_rows, int K,
+                        int H, int N, void *stream);
 
 #ifdef __cplusplus
 }

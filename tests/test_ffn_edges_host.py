@@ -119,3 +119,21 @@ def test_a_trace_into_a_graph_module_is_refused(nodes, name, how):
     call, ops = node_calls(nodes)[name]
     with pytest.raises(RuntimeError, match='cannot be traced'):
         make_fx(call, **how)(*ops)
+
+
+def test_column_sums_are_refused_before_a_launch(nodes):
+    """of f32, without room or a host number for them, more of them than there can be"""
+    import ctypes as C
+    lib, p, n = N.lib(), C.c_void_p(4096), None      # (4096 is never read)
+    num = C.c_int64(7)
+    need = lib.arcn_bias_sums_floats(200, 8)
+    assert need >= 4 * 8 and lib.arcn_bias_sums_floats(0, 8) == 0 and lib.arcn_bias_sums_floats(-1, 8) == 0 and lib.arcn_bias_sums_floats(1, 0) == 0
+    dz = lambda sums, room, at, dtype: lib.arcn_dense_dz_sums(p, 8, p, n, p, 8, p, n, sums, room, at, dtype, 7, 1.0, 200, 8, 8, n)
+    gated = lambda sums, room, at, dtype: lib.arcn_gated_bwd_sums(p, 8, p, p, n, n, p, 8, p, p, sums, room, at, dtype, 7, 1.0, 200, 8, 4, 8, n)
+    for call in (dz, gated):
+        assert call(p, need, C.byref(num), 0) == -1
+        assert call(p, need - 1, C.byref(num), 1) == -1
+        assert call(p, need, n, 2) == -1
+    assert lib.arcn_dense_dz_sums(n, 8, n, n, n, 8, n, n, p, 0, C.byref(num), 1, 7, 1.0, 0, 8, 8, n) == 0 and num.value == 0      # no rows
+    for dtype, rows in ((0, 1), (1, -1), (1, 5)):
+        assert lib.arcn_dense_dw_sums(p, 8, p, 8, p, rows, p, p, dtype, p, 1 << 20, 200, 8, 8, n) == -1

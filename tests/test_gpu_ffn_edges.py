@@ -235,12 +235,16 @@ def test_dense_calls_are_the_nodes(dtype, rows, k, n):
         y = A.linear_act_residual(xg, w, b, r, act=act, beta=2.0)
         same((F.dense_fwd(x, wd, bd, r, act, 2.0),), (y.detach(),))
         want = torch.autograd.grad(y, [xg, w, b], dy)
-        dz, dx = F.dense_dz(x, wd, bd, dy, act, 2.0, want_dx=True)
-        same((dx,) + F.dense_dw(dz, x, want_db=True), want)
-        same(F.dense_dw(dz, x), (want[1], None))
+        dz, dx, sums = F.dense_dz(x, wd, bd, dy, act, 2.0, want_dx=True, want_sums=True)
+        assert (sums is not None) == (rows > 0 and act is not None and dtype != torch.float32)
+        same((dx,) + F.dense_dw(dz, x, True, sums), want)
+        same(F.dense_dw(dz, x, sums=sums), (want[1], None))
+        same(F.dense_dz(x, wd, bd, dy, act, 2.0, want_dx=True) + F.dense_dw(dz, x), (dz, dx, want[1], None))
         if act is None or rows < 16384:                                     # (else dx comes from the kernel of dz, in another order of sums)
             alone = F.dense_dz(x, wd, bd, dy, act, 2.0)
             same((alone, F.dense_dx(alone, wd)), (dz, dx))
+            alone, some = F.dense_dz(x, wd, bd, dy, act, 2.0, want_sums=True)
+            same((alone, some), (dz, sums))
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
@@ -256,8 +260,9 @@ def test_gated_calls_are_the_nodes(dtype, rows, k, hid, n):
     h = F.gated_fwd(x, q['wg'], q['wu'], q['bg'], q['bu'])
     same((F.dense_fwd(h, q['wd'], q['bd'], r),), (y.detach(),))
     want = dict(zip(['x'] + list(p), torch.autograd.grad(y, [xg] + list(p.values()), dy)))
-    dgu = F.gated_bwd(x, q['wg'], q['wu'], q['bg'], q['bu'], dy, q['wd'])
-    dw, db = F.dense_dw(dgu, x, want_db=True)
+    dgu, sums = F.gated_bwd(x, q['wg'], q['wu'], q['bg'], q['bu'], dy, q['wd'], want_sums=True)
+    same((F.gated_bwd(x, q['wg'], q['wu'], q['bg'], q['bu'], dy, q['wd']),), (dgu,))
+    dw, db = F.dense_dw(dgu, x, True, sums)
     same((F.dense_dx(dgu, q['wg'], q['wu']), dw[:hid], dw[hid:], db[:hid], db[hid:]) + F.dense_dw(dy, h, want_db=True),
          tuple(want[name] for name in ('x', 'wg', 'wu', 'bg', 'bu', 'wd', 'bd')))
 
@@ -268,6 +273,8 @@ def test_calls_without_autograd_refuse():
     bad = [lambda: F.layer_norm_bwd(x, x, None, st, param_dtype=torch.float64), lambda: F.layer_norm_bwd(x, x, None, st, param_dtype=torch.bfloat16),
            lambda: F.layer_norm_bwd(x, x, None, st[:3]), lambda: F.layer_norm_bwd(x, x, None, st.half()), lambda: F.layer_norm_bwd(x, x[:3], None, st),
            lambda: F.layer_norm_bwd(x, x, torch.ones(7, device='cuda'), st), lambda: F.dense_dz(x, w, None, x, 'silu'), lambda: F.dense_dz(x, w, None, x[:, :6].half(), 'silu'),
+           lambda: F.dense_dw(x, x, True, torch.zeros(1, 7, device='cuda')), lambda: F.dense_dw(x, x, True, torch.zeros(1, 8, device='cuda')),
+           lambda: F.dense_dw(x.half(), x.half(), True, torch.zeros(2, 8, device='cuda')), lambda: F.dense_dw(x.half(), x.half(), True, torch.zeros(1, 8, device='cuda').half()),
            lambda: F.dense_dx(x, w), lambda: F.dense_dx(x[:, :7], w[:3], w[:3]), lambda: F.dense_dx(x, w[:4], w[:3]), lambda: F.dense_dw(x, x[:3]),
            lambda: F.gated_fwd(x, w, w[:5]), lambda: F.gated_bwd(x, w, w, None, None, x, torch.zeros(8, 5, device='cuda')),
            lambda: F.gated_bwd(x, w, w, None, None, x[:, :7], torch.zeros(8, 6, device='cuda'))]
@@ -310,8 +317,9 @@ def test_dense_sums_are_exact(dtype, rows, k, n):
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
 @pytest.mark.parametrize('rows,k,hid,n', [(1, 1, 1, 1), (300, 24, 40, 16), (8301, 130, 260, 136), (33000, 264, 520, 264), (50001, 256, 264, 256)])
 def test_gated_sums_are_exact(dtype, rows, k, hid, n):
-    """the block without an activation, all of it integers: h = g u, du = dh g and dg = dh u are rounded to the type, every result once.  Sums of
-    k <= 264 terms are below 2^9, h below 2^18, dh below 2^9 (n <= 264) and the others far inside 2^24 (random signs: 2^8.5 sqrt(33000))."""
+    """the block without an activation, all of it integers: h = g u, du = dh g and dg = dh u are rounded to the type (the bias gradients are the sums of
+    what they were before), every result once.  Sums of k <= 264 terms are below 2^9, h below 2^18, dh below 2^9 (n <= 264) and the others far
+    inside 2^24 (random signs: 2^8.5 sqrt(33000))."""
     from arcnerf_amd.ops import autograd as A
     x, dy, r = ints(1, rows, k, dtype=dtype), ints(2, rows, n, dtype=dtype), ints(3, rows, n, dtype=dtype)
     wg, wu, wd = ints(4, hid, k, dtype=dtype), ints(5, hid, k, dtype=dtype), ints(6, n, hid, dtype=dtype)
@@ -322,9 +330,28 @@ def test_gated_sums_are_exact(dtype, rows, k, hid, n):
     g, u, dh = exact(x, wg.t()) + bg.double(), exact(x, wu.t()) + bu.double(), exact(dy, wd)
     h, dg, du = ((a * b).to(dtype).double() for a, b in ((g, u), (dh, u), (dh, g)))
     assert torch.equal(y.detach(), (exact(h, wd.t()) + bd.double() + r.double()).to(dtype))
-    want = (exact(dg, wg) + exact(du, wu), exact(dg.t(), x), exact(du.t(), x), exact(dy.t(), h), dg.sum(0), du.sum(0), dy.double().sum(0))
+    want = (exact(dg, wg) + exact(du, wu), exact(dg.t(), x), exact(du.t(), x), exact(dy.t(), h), (dh * u).sum(0), (dh * g).sum(0), dy.double().sum(0))
     for name, a, b in zip(('dx', 'dwg', 'dwu', 'dwd', 'dbg', 'dbu', 'dbd'), got, want):
         assert torch.equal(a, b.to(dtype)), name
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+@pytest.mark.parametrize('rows,k,n', [(3, 8, 16), (1001, 24, 40), (1001, 25, 41), (16500, 64, 136), (33001, 129, 130), (40003, 256, 256), (70001, 100, 500), (33100, 520, 520)])
+def test_bias_gradient_has_no_rounded_terms(dtype, rows, k, n):
+    """weights of zero: dz = dy act'(b), the same digits in every row, which a 16-bit dz rounds the same way every time.  The sum is rounded once; its
+    terms carry 24 e (e = 2^-24) of the slope and the product, and no chain of its additions is longer than 256."""
+    from arcnerf_amd.ops import autograd as A
+    b = torch.linspace(-3, 3, n).to(dtype)
+    dy = ints(1, rows, n, dtype=dtype).abs() + 1
+    w = torch.zeros(n, k, dtype=dtype, device='cuda', requires_grad=True)
+    x, bg = ints(2, rows, k, dtype=dtype).requires_grad_(True), b.cuda().requires_grad_(True)
+    y = A.linear_act_residual(x, w, bg, act='sigmoid')
+    s = torch.sigmoid(b.double()) * torch.sigmoid(-b.double())
+    want = s * dy.double().sum(0).cpu()
+    tol = torch.finfo(dtype).eps / 2 * want + (256 + 24) * E24 * want
+    for leaves in ([x, w, bg], [bg]):
+        db = torch.autograd.grad(y, leaves, dy, retain_graph=True)[-1].double().cpu()
+        assert ((db - want).abs() <= tol).all(), ((db - want).abs() / tol).max().item()
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
