@@ -13,7 +13,7 @@
 // at K = 256 a tile computes it faster than HBM would return it).  The gated backward computes g, u AND dh of a tile in registers; only
 // dg and du, each rounded once, are written.  (That rounding, and h's and dz's, are the 16-bit types' only ones between a call's inputs and
 // its results: dx and dW are made from the rounded values, which costs them as much again as their own rounding, 1.4 x in all; in f32 these
-// tensors would be twice the traffic and the products three times the operations.  The bias gradients are sums of the values before that.)
+// tensors would be twice the traffic and the products six times the operations.  The bias gradients are sums of the values before that.)
 //
 // f32 operands are split into three bf16 planes on their way into LDS, x = hi + mid + lo, and six products (hi hi, hi mid, mid hi, hi lo,
 // lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  416 TFLOP/s of f32-accurate products against 157
@@ -456,6 +456,16 @@ dense_kernel(const DenseArgs<T> p) {
     const bool given_sums = SUM_MMA && p.want_sums && i0 == 0 && p.sums;
     const bool my_sums = MODE == kDenseDw && p.want_sums && i0 == 0 && (wi == 0 || SUM_ADD) && !given_sums;   // wave-uniform
 
+    // given column sums: the slab's share of their rows, THREADS / BJ threads to a column (in front of the product, which hides the loads)
+    float given = 0.f;
+    if constexpr (SUM_MMA) {
+        if (given_sums && j0 + tid % BJ < p.j.n_out) {
+            const int64_t lo = p.n_sums * slab / p.slabs, hi = p.n_sums * (slab + 1) / p.slabs;
+#pragma unroll 4
+            for (int64_t k = lo + tid / BJ; k < hi; k += THREADS / BJ) given += p.sums[k * p.j.n_out + j0 + tid % BJ];
+        }
+    }
+
     // after the swap a lane holds 8 features of a pair of tiles from 32 pr + f8, row o
     const int g = lane >> 4, o = lane & 15, f8 = 16 * (g & 1) + 8 * (g >> 1);
     // residual (or dy) of the lane's results.  16-bit types with registers to spare fetch it in front of the product, which hides the
@@ -628,21 +638,15 @@ dense_kernel(const DenseArgs<T> p) {
             if (SUM_MMA && my_sums && g == 0 && j < p.j.n_out) part[p.i.n_out * p.j.n_out + j] = sums[n][0];
         }
         if constexpr (SUM_MMA) {
-            if (given_sums) {      // the slab's share of them: THREADS / BJ threads to a column
-                const int64_t lo = p.n_sums * slab / p.slabs, hi = p.n_sums * (slab + 1) / p.slabs, j = j0 + tid % BJ;
-                float v = 0.f;
-                if (j < p.j.n_out) {
-#pragma unroll 8
-                    for (int64_t k = lo + tid / BJ; k < hi; k += THREADS / BJ) v += p.sums[k * p.j.n_out + j];
-                }
+            if (given_sums) {
                 float *f = reinterpret_cast<float *>(lds);      // behind the product's last barrier
-                f[tid] = v;
+                f[tid] = given;
                 __syncthreads();
-                if (tid < BJ && j < p.j.n_out) {
-                    v = 0.f;
+                if (tid < BJ && j0 + tid < p.j.n_out) {
+                    float v = 0.f;
 #pragma unroll
                     for (int k = 0; k < THREADS / BJ; ++k) v += f[k * BJ + tid];
-                    part[p.i.n_out * p.j.n_out + j] = v;
+                    part[p.i.n_out * p.j.n_out + j0 + tid] = v;
                 }
             }
         }
@@ -938,7 +942,7 @@ dense_dz_dx_kernel(const DenseArgs<T> p) {
                         for (int e = 0; e < 8; ++e) v[e] = n0 + 32 * pr + f8 + e < N ? v[e] : 0.f;
                     }
                     dy[pr] = Elem<T>::pack(v);      // dz from here on
-                    if (p.sums) {
+                    if (p.sums && n0 + 32 * pr < N) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[e] = sum16(live ? v[e] : 0.f);
                         if (o == 0) {

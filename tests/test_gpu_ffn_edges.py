@@ -558,3 +558,32 @@ def test_weight_gradient_of_more_elements_than_a_launch_has_threads():
     assert torch.equal(db, dz[0])
     for a in range(0, n, 8192):
         assert torch.equal(dw[a:a + 8192], dz[0, a:a + 8192, None] * x)
+
+
+# ---- captured passes ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', TYPES, ids=IDS)
+def test_training_passes_with_biases_replay(dtype):
+    """a gated block and a dense layer with all their biases, whose column sums are a buffer of the pass: replays with other inputs, eager passes of
+    the same shapes in between, are the eager results"""
+    from arcnerf_amd.ops import autograd as A
+    rows, k, hid = 16500, 40, 72
+    p = [leaf(j, *s, dtype=dtype, scale=0.2) for j, s in enumerate([(hid, k), (hid, k), (k, hid), (hid,), (hid,), (k,), (k, k), (k,)])]
+    xs, dy = [leaf(20 + j, rows, k, dtype=dtype).detach() for j in range(3)], leaf(30, rows, k, dtype=dtype).detach()
+
+    def run(x):
+        x = x.detach().requires_grad_(True)
+        y = A.linear_act_residual(A.gated_ffn(x, *p[:6], residual=x), p[6], p[7], act='gelu')
+        return (y.detach(),) + torch.autograd.grad(y, [x] + p, dy)
+
+    want = [run(x) for x in xs]
+    held = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(held)
+    for trip in range(4):
+        held.copy_(xs[trip % 3])
+        graph.replay()
+        eager = run(xs[(trip + 1) % 3])
+        torch.cuda.synchronize()
+        same(out, want[trip % 3])
+        same(eager, want[(trip + 1) % 3])
