@@ -8,16 +8,19 @@
 // reads) or its output index contiguous (TR: the weights of an input gradient, both operands of a weight gradient: fragments are
 // transposing LDS reads, ds_read_b64_tr_b16), so nothing is ever transposed in memory.
 //
-// Nothing of the forward pass but its inputs (and h) is kept for the backward: a pre-activation is computed again in the tile that needs
-// its slope, in f32, where a saved one would have been rounded to the layer's type and cost its bytes twice (2 K operations per 4 bytes:
-// at K = 256 a tile computes it faster than HBM would return it).  The gated backward computes g, u AND dh of a tile in registers; only
+// Nothing of the forward pass but its inputs (and h) is kept for the backward: a pre-activation is computed again, in f32, in the tile that
+// needs its slope.  A 16-bit layer's saved one would have been rounded to its type and cost its bytes twice (2 K operations per 4 bytes: at
+// K = 256 a tile computes it faster than HBM would return it).  An f32 layer loses nothing by saving it and pays for the product from K of
+// about 160 on (at 256 2.7 ps an element at the split products' rate below against 1.7 for its 8 bytes): what it gets is the memory.  The
+// gated backward computes g, u AND dh of a tile in registers; only
 // dg and du, each rounded once, are written.  (That rounding, and h's and dz's, are the 16-bit types' only ones between a call's inputs and
 // its results: dx and dW are made from the rounded values, which costs them as much again as their own rounding, 1.4 x in all; in f32 these
 // tensors would be twice the traffic and the products six times the operations.  The bias gradients are sums of the values before that.)
 //
 // f32 operands are split into three bf16 planes on their way into LDS, x = hi + mid + lo, and six products (hi hi, hi mid, mid hi, hi lo,
-// lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  416 TFLOP/s of f32-accurate products against 157
-// on the f32 MFMA.  Infinities and NaN in such an operand give NaN.
+// lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  A sixth of the bf16 rate, 193 TFLOP/s at the 1156 of a
+// large library product here, whose f32 products reach 154; the gated forward 32768 x 256 -> 2 x 512 runs at 155 (111 us).  Infinities, NaN and
+// what rounds to infinity as bf16 (from 3.39e38 on) in such an operand give NaN.
 //
 // A lane's accumulators of one MFMA tile are 4 consecutive features of a row; the tiles are taken in pairs and lane rows 1 and 3 of the
 // first are swapped with lane rows 0 and 2 of the second (v_permlane16_swap_b32), which leaves 8 CONSECUTIVE features of one row in each
@@ -1003,17 +1006,18 @@ dense_dz_dx_kernel(const DenseArgs<T> p) {
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------------
-// dense_few_kernel: as long as two of its workgroups to a CU (f32: eight) do the product.  One feature block of it costs 3 - 5 us whatever the
-// rows, the tiles' first step waits longer and in f32 computes six products on a few CUs: 256 x 256 bf16 3.5 us at 512 rows (tiles 4.4), f32
-// 4.7 (11.1); 1024 x 1024 bf16 5.3 at 128 rows and 13.2 at 512 (7.9), f32 8.6 and 24 (34).
+// dense_few_kernel: as long as two of its workgroups to a CU (f32: four) do the product.  One feature block of it costs 3 - 5 us whatever the rows,
+// the tiles' first step waits longer and in f32 computes six products on a few CUs.  us here / by tiles, 1024 outputs, at the limit and at twice
+// that, reductions of 32, 256, 1024, 4096:  bf16, 256 rows 3.1 / 4.0, 4.1 / 4.4, 8.0 / 7.8, 24 / 34, 512 rows 3.3 / 4.1, 5.5 / 4.5, 13 / 7.9, 45 / 34;
+// f32, 512 rows 4.1 / 4.8, 8.8 / 11, 25 / 35, 87 / 124, 1024 rows 6.0 / 5.2, 15 / 12, 46 / 35, 170 / 125.
 static inline bool dense_few(int elem_bytes, int64_t rows, int64_t n) {
-    return rows <= 1024 && ceil_div<int64_t>(n, 16) * ceil_div<int64_t>(rows, 32) <= (elem_bytes == 2 ? 512 : 2048);
+    return rows <= 1024 && ceil_div<int64_t>(n, 16) * ceil_div<int64_t>(rows, 32) <= (elem_bytes == 2 ? 512 : 1024);
 }
 
-
-// dense_dz_dx_kernel's layers: 16 bits, enough rows for the weight that every CU loads first
-// (16384 rows: 63 -> 40, 20000 rows 13 us against 9 + 9 of which one launch is 3)
-constexpr int64_t kStayRows = 16384;
+// dense_dz_dx_kernel's layers: 16 bits, enough rows for the weight that every CU loads first.  us here / as two products, with the column sums,
+// 16384, 24576, 32768 and 65536 rows:  16 -> 16 8.3 / 8.8, 8.4 / 9.6, 8.6 / 12, 16 / 15;  64 -> 64 8.4 / 7.2, 8.8 / 8.4, 9.1 / 15, 16 / 20;
+// 128 -> 128 11 / 9.8, 11 / 12, 13 / 16, 23 / 25;  128 -> 512 28 / 24, 30 / 31, 31 / 39, 52 / 62.
+constexpr int64_t kStayRows = 24576;
 template <typename T>
 static bool dense_stays(int64_t rows, int K, int N) {
     return sizeof(T) == 2 && K >= 8 && N >= 8 && K <= 128 && N <= 512 && rows >= kStayRows;

@@ -868,8 +868,9 @@ def _host_act(z, code, beta):
 
 def linear_act_residual(x, weight, bias=None, residual=None, act=None, beta=1.0):
     """act(x @ weight.T + bias) + residual as one product with an epilogue: x (..., K), weight (N, K), bias (N), residual (..., N) like the
-    result; one type for all of them, float32, bfloat16 or float16.  act: None, relu, sigmoid, softplus (beta), silu, gelu.  Infinities and NaN in
-    float32 operands give NaN."""
+    result; one type for all of them, float32, bfloat16 or float16.  act: None, relu, sigmoid, softplus (beta), silu, gelu.  Infinities, NaN and
+    numbers from 3.39e38 on in float32 operands give NaN.  In the backward the pre-activation's gradient is held in the layer's type (float16: it
+    has to stay in range); the bias's gradient is summed before that rounding."""
     code = F._dense_act(act, beta)
     if not x.is_cuda:
         y = _host_act(torch.nn.functional.linear(x, weight, bias), code, beta)
@@ -879,7 +880,8 @@ def linear_act_residual(x, weight, bias=None, residual=None, act=None, beta=1.0)
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, residual=None, act='silu', beta=1.0):
     """The gated feed-forward block (act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)) @ w_down.T + b_down + residual: x (..., K), w_gate and
-    w_up (H, K), w_down (N, H), residual (..., N); one type for all of them, in which the product of the gate is held too."""
+    w_up (H, K), w_down (N, H), residual (..., N); one type for all of them, in which the product of the gate is held too, and in the backward the
+    gradients of its two factors (float16: they have to stay in range); the biases' gradients are summed before that rounding."""
     code = F._dense_act(act, beta)
     if not x.is_cuda:
         lin = torch.nn.functional.linear

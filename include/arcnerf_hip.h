@@ -813,7 +813,8 @@ int arcn_ngp_step_tail(const arcn_mlp_desc *desc_a, float *scratch_a, int64_t w_
  * Residual feed-forward layers of wide nets (no counterpart in the reference, whose nets are the DenseLayer stacks of
  * arcnerf/models/base_modules/geo_rad_model/linear_network_module.py:16-335): layer norm, a dense layer with activation and residual, a
  * gated pair of dense layers; forward and first-order backward.  dtype = ARCN_DTYPE_* is the type of every `void *` tensor of a call.
- * Sums, statistics and activations are computed in f32, results are rounded once.  Rows (x, dy, dz, residual) may start at any element
+ * Sums, statistics and activations are computed in f32, results are rounded once (of a 16-bit layer dz, dgu and h are results, from which
+ * the others are made: the bias gradients by way of the *_sums calls are not).  Rows (x, dy, dz, residual) may start at any element
  * and lie ld elements apart (ld >= the width); weights, biases and outputs are contiguous.  Outputs must not overlap inputs.  The
  * reductions over rows have a fixed order: the same call gives the same bits.
  * ---------------------------------------------------------------------------------------------- */
@@ -830,7 +831,7 @@ int arcn_layer_norm_bwd(const void *x, int64_t ld_x, const void *dy, int64_t ld_
 
 /* y (n_rows, N) = act(x (n_rows, K) w (N, K)^T + bias) + residual; bias and residual may be NULL.  act = ARCN_ACT_NONE, _RELU, _SIGMOID,
  * _SOFTPLUS (beta > 0; identity from beta z > 20), _SILU, _GELU.  f32 products are accumulated from three-way bf16 splits of the operands
- * (f32 accuracy; infinities and NaN give NaN). */
+ * (f32 accuracy; infinities, NaN and numbers from 3.39e38 on give NaN). */
 int arcn_dense_fwd(const void *x, int64_t ld_x, const void *w, const void *bias, const void *residual, int64_t ld_res, void *y, int dtype, int act,
                    float beta, int64_t n_rows, int K, int N, void *stream);
 /* dz (n_rows, N) = dy act'(x w^T + bias): the gradient of the pre-activation, which is computed again from x (nothing was saved); unless dx is

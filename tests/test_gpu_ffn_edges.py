@@ -224,7 +224,7 @@ def test_layer_norm_calls_are_the_nodes(dtype, rows, width):
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
-@pytest.mark.parametrize('rows,k,n', [(1, 8, 8), (37, 45, 21), (500, 128, 72), (17000, 40, 56), (0, 16, 8)])
+@pytest.mark.parametrize('rows,k,n', [(1, 8, 8), (37, 45, 21), (500, 128, 72), (17000, 40, 56), (30000, 40, 56), (0, 16, 8)])
 def test_dense_calls_are_the_nodes(dtype, rows, k, n):
     from arcnerf_amd.ops import autograd as A, functional as F
     x, dy, r = wide_rows(1, rows, k, dtype), wide_rows(2, rows, n, dtype), wide_rows(3, rows, n, dtype)
@@ -240,7 +240,7 @@ def test_dense_calls_are_the_nodes(dtype, rows, k, n):
         same((dx,) + F.dense_dw(dz, x, True, sums), want)
         same(F.dense_dw(dz, x, sums=sums), (want[1], None))
         same(F.dense_dz(x, wd, bd, dy, act, 2.0, want_dx=True) + F.dense_dw(dz, x), (dz, dx, want[1], None))
-        if act is None or rows < 16384:                                     # (else dx comes from the kernel of dz, in another order of sums)
+        if act is None or rows < 24576:                                     # (else dx comes from the kernel of dz, in another order of sums)
             alone = F.dense_dz(x, wd, bd, dy, act, 2.0)
             same((alone, F.dense_dx(alone, wd)), (dz, dx))
             alone, some = F.dense_dz(x, wd, bd, dy, act, 2.0, want_sums=True)
@@ -297,7 +297,7 @@ def exact(a, b):
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
-@pytest.mark.parametrize('rows,k,n', [(1, 1, 1), (255, 24, 40), (1000, 7, 3), (33001, 129, 130), (16400, 128, 72), (70001, 63, 31), (17000, 256, 256), (20003, 520, 520),
+@pytest.mark.parametrize('rows,k,n', [(1, 1, 1), (255, 24, 40), (1000, 7, 3), (33001, 129, 130), (16400, 128, 72), (24577, 128, 512), (70001, 63, 31), (17000, 256, 256), (20003, 520, 520),
                                       (33100, 520, 520), (66000, 264, 264), (300007, 16, 16)])
 def test_dense_sums_are_exact(dtype, rows, k, n):
     """forward, dx, dW and db of the layer without an activation and of one whose activation is the identity (relu above zero: the kernels that compute
@@ -336,7 +336,7 @@ def test_gated_sums_are_exact(dtype, rows, k, hid, n):
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
-@pytest.mark.parametrize('rows,k,n', [(3, 8, 16), (1001, 24, 40), (1001, 25, 41), (16500, 64, 136), (33001, 129, 130), (40003, 256, 256), (70001, 100, 500), (33100, 520, 520)])
+@pytest.mark.parametrize('rows,k,n', [(3, 8, 16), (1001, 24, 40), (1001, 25, 41), (16500, 64, 136), (25001, 64, 136), (33001, 129, 130), (40003, 256, 256), (70001, 100, 500), (33100, 520, 520)])
 def test_bias_gradient_has_no_rounded_terms(dtype, rows, k, n):
     """weights of zero: dz = dy act'(b), the same digits in every row, which a 16-bit dz rounds the same way every time.  The sum is rounded once; its
     terms carry 24 e (e = 2^-24) of the slope and the product, and no chain of its additions is longer than 256."""
@@ -511,7 +511,7 @@ def test_layer_norm_keeps_rows_apart(dtype, width):
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=IDS)
-@pytest.mark.parametrize('rows,k,n', [(20, 24, 13), (300, 45, 21), (16400, 24, 13), (33001, 129, 130), (66000, 264, 264)])
+@pytest.mark.parametrize('rows,k,n', [(20, 24, 13), (300, 45, 21), (16400, 24, 13), (30001, 24, 13), (33001, 129, 130), (66000, 264, 264)])
 def test_dense_and_gated_keep_rows_apart(dtype, rows, k, n):
     from arcnerf_amd.ops import autograd as A
     x, dy, r = (leaf(j, rows, s, dtype=dtype).detach() for j, s in enumerate((k, n, n)))
@@ -566,7 +566,7 @@ def test_training_passes_with_biases_replay(dtype):
     """a gated block and a dense layer with all their biases, whose column sums are a buffer of the pass: replays with other inputs, eager passes of
     the same shapes in between, are the eager results"""
     from arcnerf_amd.ops import autograd as A
-    rows, k, hid = 16500, 40, 72
+    rows, k, hid = 30000, 40, 72
     p = [leaf(j, *s, dtype=dtype, scale=0.2) for j, s in enumerate([(hid, k), (hid, k), (k, hid), (hid,), (hid,), (k,), (k, k), (k,)])]
     xs, dy = [leaf(20 + j, rows, k, dtype=dtype).detach() for j in range(3)], leaf(30, rows, k, dtype=dtype).detach()
 
@@ -587,3 +587,11 @@ def test_training_passes_with_biases_replay(dtype):
         torch.cuda.synchronize()
         same(out, want[trip % 3])
         same(eager, want[(trip + 1) % 3])
+
+
+@pytest.mark.parametrize('dtype', TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize('rows,k,n,act,pitch', [(24576, 8, 8, 'silu', 0), (24593, 128, 128, 'gelu', 0), (26000, 100, 60, 'softplus', 3), (24600, 128, 512, 'silu', 0), (27001, 125, 13, 'sigmoid', 1)])
+def test_dense_weight_on_chip(dtype, rows, k, n, act, pitch):
+    """dz and dx of one kernel: the fewest rows that take it, partial groups of rows, widths and features that end inside a pack"""
+    from test_gpu_ffn import check_dense
+    check_dense(rows, k, n, dtype, act, pitch=pitch, bias=act != 'silu', residual=act != 'sigmoid')
