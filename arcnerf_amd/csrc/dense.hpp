@@ -12,10 +12,10 @@
 // needs its slope.  A 16-bit layer's saved one would have been rounded to its type and cost its bytes twice (2 K operations per 4 bytes: at
 // K = 256 a tile computes it faster than HBM would return it).  An f32 layer loses nothing by saving it and pays for the product from K of
 // about 160 on (at 256 2.7 ps an element at the split products' rate below against 1.7 for its 8 bytes): what it gets is the memory.  The
-// gated backward computes g, u AND dh of a tile in registers; only
-// dg and du, each rounded once, are written.  (That rounding, and h's and dz's, are the 16-bit types' only ones between a call's inputs and
-// its results: dx and dW are made from the rounded values, which costs them as much again as their own rounding, 1.4 x in all; in f32 these
-// tensors would be twice the traffic and the products six times the operations.  The bias gradients are sums of the values before that.)
+// gated backward computes g, u AND dh of a tile in registers; only dg and du, each rounded once, are written.  (That rounding, and h's and
+// dz's, are the 16-bit types' only ones between a call's inputs and its results: dx and dW are made from the rounded values, which costs
+// them as much again as their own rounding, 1.4 x in all; in f32 these tensors would be twice the traffic and the products six times the
+// operations.  The bias gradients are sums of the values before that.)
 //
 // f32 operands are split into three bf16 planes on their way into LDS, x = hi + mid + lo, and six products (hi hi, hi mid, mid hi, hi lo,
 // lo hi, mid mid) are accumulated in f32; what is dropped is below 2^-25 of a product.  A sixth of the bf16 rate, 193 TFLOP/s at the 1156 of a
@@ -850,8 +850,9 @@ dense_few_kernel(const DenseArgs<T> p) {
 // their own, 16 rows at a time, without another barrier.  A lane's fragments of x come straight from memory (its row's 16 bytes); the
 // pre-activation is computed again for 128 features at a time, and because a lane's 8 consecutive features of dz are what the next
 // product wants as its J fragment, dx = dz W follows in registers on the SAME weight, read the other way round (transposing reads).  The
-// reduction over features is dealt to the lanes as the features fell (f8).  x and dy in, dz and dx out: 128 -> 112, 317560 rows, bf16 77 us
-// (3.9 TB/s) against 67 + 47 as two products.  (With 256 inputs the accumulators of dx do not fit beside the rest: 236 us against 127 + 75.)
+// reduction over features is dealt to the lanes as the features fell (f8).  x and dy in, dz and dx out: 128 -> 112, 317560 rows, bf16 71 us
+// (4.3 TB/s) against 67 + 47 as two products, 80 with the column sums.  (With 256 inputs the accumulators of dx do not fit beside the rest: 236 us
+// against 127 + 75.)
 template <typename T, int KS>
 __global__ void __launch_bounds__(512, 2)
 dense_dz_dx_kernel(const DenseArgs<T> p) {
